@@ -18,6 +18,7 @@ from .op import (  # noqa: F401
     set_split_mode,
 )
 
+from .decode import decode_attention, decode_attention_paged  # noqa: F401,E402
 from .speculative import DraftTree, TreeVerifyAttention, accept_longest_path  # noqa: F401,E402
 
 __all__ = [
@@ -26,6 +27,8 @@ __all__ = [
     "TreeVerifyAttention",
     "accept_longest_path",
     "commit_accepted",
+    "decode_attention",
+    "decode_attention_paged",
     "flash_decoding_attention",
     "flash_decoding_attention_paged",
     "flash_decoding_attention_with_lse",

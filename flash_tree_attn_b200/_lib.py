@@ -8,6 +8,10 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
+from ctypes import byref  # noqa: F401
+
+import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # FTA_LIB_PATH points at a library built elsewhere (same ABI); the default is the in-tree build.
@@ -98,6 +102,33 @@ class FtaExchangeParams(C.Structure):
     ]
 
 
+class FtaTokenParams(C.Structure):
+    """Mirror of `struct FtaTokenParams` (include/fta.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("q_sb", _i64), ("q_sh", _i64),
+        ("k_cache", _vp), ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64),
+        ("v_cache", _vp), ("v_sb", _i64), ("v_sh", _i64), ("v_st", _i64),
+        ("kv_seq_len", _vp), ("block_table", _vp), ("bt_sb", _i64), ("slopes", _vp),
+        ("out", _vp), ("o_sb", _i64), ("o_sh", _i64), ("lse", _vp), ("l_sb", _i64),
+        ("row_weights", _vp), ("rw_sb", _i64), ("rw_sh", _i64), ("workspace", _vp), ("workspace_bytes", _i64),
+        ("sm_scale", _f32), ("softcap", _f32), ("window", _i32), ("len_is_i64", _i32),
+        ("B", _i32), ("H", _i32), ("Hkv", _i32), ("D", _i32), ("ctx", _i32),
+        ("page_size", _i32), ("n_pages", _i32), ("dtype", _i32), ("grid_override", _i32), ("reserved_", _i32),
+    ]
+
+
+def _packer(cls):
+    """The fields of one call as the bytes of the C struct, in one step: filling a ctypes structure
+    field by field costs several times as much, and a decoding step makes many small calls."""
+    code = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
+    fmt = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    assert fmt.size == C.sizeof(cls)
+    return fmt.pack
+
+
+pack_token = _packer(FtaTokenParams)
+
 # every symbol include/fta.h declares: (restype, argtypes)
 SYMBOLS = {
     "fta_version": (C.c_int, []),
@@ -110,6 +141,8 @@ SYMBOLS = {
     "fta_stage1": (C.c_int, [C.POINTER(FtaParams), _vp]),
     "fta_stage2": (C.c_int, [C.POINTER(FtaParams), _vp]),
     "fta_merge_parts": (C.c_int, [C.POINTER(FtaMergeParams), _vp]),
+    "fta_decode_token_workspace_bytes": (_i64, [_vp]),
+    "fta_decode_token": (C.c_int, [_vp, _vp]),
     "fta_commit_accepted": (C.c_int, [C.POINTER(FtaCommitParams), _vp]),
     "fta_exchange_merge": (C.c_int, [C.POINTER(FtaExchangeParams), _vp]),
     "fta_plan_host": (_i64, [C.POINTER(FtaParams), C.POINTER(_i64), C.POINTER(_i64), _i64,
@@ -160,3 +193,29 @@ class FtaError(RuntimeError):
 def check(code: int, where: str) -> None:
     if code != FTA_OK:
         raise FtaError(code, where)
+
+
+def rows_ok(t) -> bool:
+    """Whether the rows of a 4-D tensor can be copied in 16-byte pieces (16-bit elements)."""
+    a, b, c, d = t.stride()
+    return d == 1 and not (a | b | c) & 7 and not t.data_ptr() & 15
+
+
+class on_device:
+    """The current stream of a tensor's device, that device made current for the block if it is not."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, dev):
+        self.index = dev.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False

@@ -27,6 +27,11 @@ SOURCES = [
     "fta_stage1_mma_d64.cu",
     "fta_stage1_mma_d128.cu",
     "fta_stage1_mma_d256.cu",
+    "fta_token_join.cu",
+    "fta_token_d32.cu",
+    "fta_token_d64.cu",
+    "fta_token_d128.cu",
+    "fta_token_d256.cu",
 ]
 
 EXTRA = os.environ.get("FTA_EXTRA_NVCC_FLAGS", "").split()

@@ -33,10 +33,16 @@ void* g_static_scratch_ptr[64];  // device address of g_static_scratch, per devi
 
 thread_local char g_cuda_err[256] = "";
 
-int cuda_fail(cudaError_t e) {
+}  // namespace
+
+int fta_cuda_fail(cudaError_t e) {
   snprintf(g_cuda_err, sizeof(g_cuda_err), "%s: %s", cudaGetErrorName(e), cudaGetErrorString(e));
   return FTA_E_CUDA;
 }
+
+namespace {
+
+int cuda_fail(cudaError_t e) { return fta_cuda_fail(e); }
 
 bool aligned(const void* ptr, size_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0; }
 bool mult(int64_t v, int64_t m) { return v % m == 0; }

@@ -211,6 +211,9 @@ __host__ __device__ __forceinline__ bool fta_row(const FtaParams& p, const FtaGe
   return hh < g.hpt && gi < (p.H / p.Hkv) && qi < p.Q;
 }
 
+// Keeps the text of a CUDA error for fta_last_cuda_error and returns FTA_E_CUDA (fta_api.cu).
+int fta_cuda_fail(cudaError_t e);
+
 #ifdef __CUDACC__
 // ---- device helpers ----------------------------------------------------------------------
 

@@ -1,0 +1,202 @@
+// Joins the pieces of the one-token attention (fta_token.cuh), finishes the rows of empty sequences
+// and adds the softmax weights of the group's heads to row_weights.
+//
+// out = sum_i 2^(l_i - M) o_i / sum_i 2^(l_i - M) over the pieces' log2 LSEs l_i.  Row weights:
+// w_r += sum_h 2^(s_hr - LSE_h) from the scores stage 1 kept, so K is not read a second time
+// (4 G bytes a row instead of 2 D).
+//
+// grid = (B * Hkv, chunks of the cache's length): every block of a (sequence, KV head) works the
+// heads' LSEs out for itself, chunk 0 joins the outputs as well.
+#include "fta_token.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+__global__ void __launch_bounds__(kThreads) token_join_kernel(const FtaTokenParams p, const FtaGeom g, const int chunk_rows) {
+  __shared__ float s_lse[FTA_MAX_GROUP];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / p.Hkv, kvh = blockIdx.x - b * p.Hkv;
+  const int G = p.H / p.Hkv, lanes = g.lanes > 0 ? g.lanes : 1;
+  const bool weights = p.row_weights != nullptr;
+  const FtaTokenWs ws = fta_token_ws(g.grid, g.R, p.D, p.B, g.U, p.H, p.ctx, weights);
+  const uint8_t* wsb = reinterpret_cast<const uint8_t*>(p.workspace);
+  const float* part_o = reinterpret_cast<const float*>(wsb + ws.part_o);
+  const float* part_l = reinterpret_cast<const float*>(wsb + ws.part_l);
+  const float* lse2 = reinterpret_cast<const float*>(wsb + ws.lse2);
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx);
+  const int row0 = blockIdx.y * chunk_rows;
+  if (blockIdx.y > 0 && row0 >= L) return;
+
+  for (int hh = warp; hh < G; hh += kThreads / 32) {
+    const int gt = hh / g.R, r = hh - gt * g.R, h = kvh * G + hh;
+    const int j = kvh * g.n_gt + gt;
+    float total = -INFINITY;
+    int2 d = make_int2(0, 0);
+    if (L > 0) d = reinterpret_cast<const int2*>(wsb + ws.desc)[(long long)b * g.U + j];
+    if (d.x == 1) {  // stage 1 wrote the rows itself
+      if (weights) total = lse2[(long long)b * p.H + h];
+    } else if (d.x > 1) {
+      const int lane_of = g.lanes > 1 ? gt : 0;
+      auto slot = [&](int i) { return (long long)2 * ((d.y + i) * lanes + lane_of) + (i == 0 ? 1 : 0); };
+      // lane i holds pieces i, i + 32, ...: the largest LSE, then the weights' sum
+      float top = -INFINITY, sum = 0.f;
+      for (int i = lane; i < d.x; i += 32) {
+        const float x = part_l[slot(i) * g.R + r];
+        top = x != x ? x : fmaxf(top, x);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float x = __shfl_xor_sync(0xffffffffu, top, o);
+        top = top != top || x != x ? NAN : fmaxf(top, x);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      for (int i = lane; i < d.x; i += 32) sum += fta_exp2(part_l[slot(i) * g.R + r] - base);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      total = sum == 0.f ? -INFINITY : base + fta_log2(sum);
+      if (blockIdx.y == 0) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int c4 = lane * 4; c4 < p.D; c4 += 128) {
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int i = 0; i < d.x; ++i) {
+            const float w = fta_exp2(part_l[slot(i) * g.R + r] - base) * inv;
+            const float4 x = *reinterpret_cast<const float4*>(part_o + (slot(i) * g.R + r) * p.D + c4);
+            acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+          }
+          fta_store4(p.out, p.dtype, b * p.o_sb + h * p.o_sh + c4, acc);
+        }
+        if (lane == 0 && p.lse) p.lse[b * p.l_sb + h] = total * FTA_LN2;
+      }
+    } else if (blockIdx.y == 0) {  // no rows
+      for (int c4 = lane * 4; c4 < p.D; c4 += 128) fta_store4(p.out, p.dtype, b * p.o_sb + h * p.o_sh + c4, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (lane == 0 && p.lse) p.lse[b * p.l_sb + h] = -INFINITY;
+    }
+    if (weights && lane == 0) s_lse[hh] = total;
+  }
+  if (!weights) return;
+  __syncthreads();
+  const float* scores = reinterpret_cast<const float*>(wsb + ws.scores) + ((long long)b * p.H + kvh * G) * p.ctx;
+  float* out = p.row_weights + b * p.rw_sb + kvh * p.rw_sh;
+  const int first = max(row0, p.window > 0 ? L - p.window : 0), end = min(L, row0 + chunk_rows);
+  for (int row = first + threadIdx.x; row < end; row += kThreads) {
+    float w = 0.f;
+    for (int hh = 0; hh < G; ++hh) {
+      const float x = s_lse[hh];
+      w += x == -INFINITY ? 0.f : fta_exp2(scores[(long long)hh * p.ctx + row] - x);
+    }
+    out[row] += w;
+  }
+}
+
+template <typename F>
+int token_variant(const FtaTokenParams& p, F&& f) {
+  switch (p.D) {
+    case 32: return f(fta_launch_token_d32);
+    case 64: return f(fta_launch_token_d64);
+    case 128: return f(fta_launch_token_d128);
+  }
+  return f(fta_launch_token_d256);
+}
+
+bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+
+int check_sizes(const FtaTokenParams* p) {
+  if (!p || p->B <= 0 || p->H <= 0 || p->Hkv <= 0 || p->ctx < 0 || p->H % p->Hkv != 0) return FTA_E_BADARG;
+  if (p->D != 32 && p->D != 64 && p->D != 128 && p->D != 256) return FTA_E_BADARG;
+  if (p->dtype != FTA_DTYPE_F16 && p->dtype != FTA_DTYPE_BF16) return FTA_E_BADARG;
+  if (p->grid_override < 0) return FTA_E_BADARG;
+  if (p->B > FTA_MAX_BATCH || p->H / p->Hkv > FTA_MAX_GROUP) return FTA_E_UNSUPPORTED;
+  return FTA_OK;
+}
+
+int check(const FtaTokenParams* p) {
+  if (int rc = check_sizes(p)) return rc;
+  if (!p->q || !p->kv_seq_len || !p->out || (p->ctx > 0 && (!p->k_cache || !p->v_cache))) return FTA_E_BADARG;
+  if (!aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->out)) return FTA_E_BADARG;
+  for (int64_t s : {p->q_sb, p->q_sh, p->k_sb, p->k_sh, p->k_st, p->v_sb, p->v_sh, p->v_st})
+    if (s % 8 != 0) return FTA_E_BADARG;
+  if (p->o_sb % 4 != 0 || p->o_sh % 4 != 0) return FTA_E_BADARG;
+  if (!(p->softcap >= 0.f) || p->window < 0) return FTA_E_BADARG;
+  if (p->block_table) {
+    if (p->page_size < FTA_TILE || p->page_size % FTA_TILE != 0 || p->n_pages < 1 || p->bt_sb < 0) return FTA_E_BADARG;
+    if ((long long)p->bt_sb * p->page_size < p->ctx && p->B > 1) return FTA_E_BADARG;
+  }
+  if (!p->workspace || !aligned16(p->workspace)) return FTA_E_WORKSPACE;
+  return FTA_OK;
+}
+
+// [device][dtype][head_dim][rows][KB of the prefix table] -> resident blocks per SM, 0: not asked yet
+int g_occ[16][2][4][2][34];
+int g_sms[16];
+
+int geometry(const FtaTokenParams& p, FtaGeom& g) {
+  const int G = p.H / p.Hkv;
+  // 16 padded heads cost twice the products and accumulators of 8: only where a group has more than 8,
+  // and not at head_dim 256, whose accumulators would spill; there two blocks share the rows through L2
+  g.R = G > 8 && p.D < 256 ? 16 : 8;
+  g.qpt = 1; g.n_qt = 1;
+  g.hpt = g.R;
+  g.n_gt = fta_cdiv(G, g.R);
+  g.mtiles = g.n_gt;
+  g.U = p.Hkv * g.n_gt;
+  g.n_tree = 0;
+  g.min_per = 1;
+  g.fixed_max_splits = 0; g.family = 0; g.cs = 1;
+  g.pad = 1;
+  g.grid = p.grid_override;
+  if (p.grid_override == 0) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return fta_cuda_fail(e);
+    int& sms = g_sms[dev & 15];
+    if (sms == 0 && (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return fta_cuda_fail(e);
+    const int d = p.D == 32 ? 0 : p.D == 64 ? 1 : p.D == 128 ? 2 : 3;
+    int& occ = g_occ[dev & 15][p.dtype][d][g.R == 16][((p.B + 1) * 4) / 1024];
+    if (occ == 0) {
+      int n = 0;
+      e = (cudaError_t)token_variant(p, [&](auto launch) { return (int)launch(p, g, 0, 1, &n); });
+      if (e != cudaSuccess) return fta_cuda_fail(e);
+      if (n < 1) return FTA_E_UNSUPPORTED;
+      occ = n;
+    }
+    g.grid = sms * occ;
+  }
+  g.lanes = g.mtiles > 1 && g.grid >= g.mtiles ? g.mtiles : 1;
+  return FTA_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t fta_decode_token_workspace_bytes(const FtaTokenParams* p) {
+  if (int rc = check_sizes(p)) return -rc;
+  FtaGeom g;
+  if (int rc = geometry(*p, g)) return -rc;
+  return fta_token_ws(g.grid, g.R, p->D, p->B, g.U, p->H, p->ctx, p->row_weights != nullptr).bytes;
+}
+
+extern "C" int fta_decode_token(const FtaTokenParams* p, void* stream) {
+  if (int rc = check(p)) return rc;
+  FtaGeom g;
+  if (int rc = geometry(*p, g)) return rc;
+  const bool weights = p->row_weights != nullptr;
+  if (p->workspace_bytes < fta_token_ws(g.grid, g.R, p->D, p->B, g.U, p->H, p->ctx, weights).bytes) return FTA_E_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e = (cudaError_t)token_variant(*p, [&](auto launch) { return (int)launch(*p, g, st, 0, nullptr); });
+  if (e != cudaSuccess) return fta_cuda_fail(e);
+  const int chunk = 2048;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p->B * p->Hkv, weights ? (p->ctx + chunk - 1) / chunk + (p->ctx == 0) : 1);
+  cfg.blockDim = dim3(kThreads); cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, token_join_kernel, *p, g, chunk);
+  return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
+}

@@ -244,6 +244,54 @@ typedef struct FtaCommitParams {
 
 int fta_commit_accepted(const FtaCommitParams* p, void* stream);
 
+/*
+ * Attention of ONE new token per sequence over the cache (the decoding step without a draft tree).
+ * The new token's own key and value are already in the cache (fta_append_tokens), so that
+ * sequence b attends to rows r of [max(0, L - window), L), L = kv_seq_len[b]:
+ *   s = sm_scale * q.k_r;  softcap > 0: s = softcap * tanh(s / softcap);
+ *   slopes: s += slopes[h] * (r - (L - 1));  out = sum_r softmax(s)_r * v_r
+ * The reference has no such entry; shapes, strides and the page table are FtaParams' with Q = 1.
+ *   row_weights  optional fp32 [B, Hkv, ctx], unit stride along ctx: row r of KV head kvh gains the
+ *                softmax weights that the group's G query heads gave it (updated in place, by one
+ *                thread per row in a fixed order: equal inputs give equal bits)
+ * An empty sequence gives out = 0, lse = -inf.  A page index outside [0, n_pages) takes the rows
+ * of that page out of the attention; nothing outside the pool is read.
+ */
+typedef struct FtaTokenParams {
+  const void* q; /* [B, H, D] */
+  int64_t q_sb, q_sh;
+  const void* k_cache;
+  int64_t k_sb, k_sh, k_st;
+  const void* v_cache;
+  int64_t v_sb, v_sh, v_st;
+  const void* kv_seq_len;     /* [B] int32 or int64 */
+  const int32_t* block_table; /* NULL: dense cache */
+  int64_t bt_sb;
+  const float* slopes; /* optional [H] */
+  void* out;           /* [B, H, D] of dtype */
+  int64_t o_sb, o_sh;
+  float* lse; /* optional [B, H], natural log */
+  int64_t l_sb;
+  float* row_weights;
+  int64_t rw_sb, rw_sh;
+  void* workspace;
+  int64_t workspace_bytes;
+  float sm_scale;
+  float softcap;  /* 0: none */
+  int32_t window; /* 0: none */
+  int32_t len_is_i64;
+  int32_t B, H, Hkv, D, ctx;
+  int32_t page_size, n_pages;
+  int32_t dtype;
+  int32_t grid_override; /* 0 = planner's choice; else blocks to launch (tests) */
+  int32_t reserved_;
+} FtaTokenParams;
+
+/* Bytes of workspace the call needs on the current device; negative: -FTA_E_*.  Sizes, dtype,
+   grid_override and whether row_weights is NULL are read. */
+int64_t fta_decode_token_workspace_bytes(const FtaTokenParams* p);
+int fta_decode_token(const FtaTokenParams* p, void* stream);
+
 /* Text for an FTA_E_* code.  No counterpart in the reference (it raises AssertionError,
    flash_tree_attn.py:263-291). */
 const char* fta_strerror(int code);
