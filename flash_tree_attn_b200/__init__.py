@@ -18,7 +18,9 @@ from .op import (  # noqa: F401
     set_split_mode,
 )
 
-from .decode import decode_attention, decode_attention_paged  # noqa: F401,E402
+from .decode import decode_attention, decode_attention_paged, evict_rows  # noqa: F401,E402
+from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401,E402
+from .rotary import append_tokens, apply_rotary, rotary_frequencies  # noqa: F401,E402
 from .speculative import DraftTree, TreeVerifyAttention, accept_longest_path  # noqa: F401,E402
 
 __all__ = [
@@ -26,15 +28,21 @@ __all__ = [
     "DraftTree",
     "TreeVerifyAttention",
     "accept_longest_path",
+    "append_tokens",
+    "apply_rotary",
     "commit_accepted",
     "decode_attention",
     "decode_attention_paged",
+    "evict_rows",
     "flash_decoding_attention",
     "flash_decoding_attention_paged",
     "flash_decoding_attention_with_lse",
     "merge_partials",
     "prepare",
+    "rotary_frequencies",
     "set_split_mode",
     "set_kernel",
     "set_grid_override",
+    "token_logprobs",
+    "TokenLogprobs",
 ]

@@ -29,6 +29,7 @@ FTA_E_TOO_LARGE = 5
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 SPLIT_BALANCED, SPLIT_FIXED = 0, 1
 KERNEL_AUTO, KERNEL_MMA, KERNEL_UMMA = 0, 1, 2
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 _i64, _i32, _vp, _f32 = C.c_int64, C.c_int32, C.c_void_p, C.c_float
 
@@ -118,16 +119,59 @@ class FtaTokenParams(C.Structure):
     ]
 
 
+class FtaRotaryParams(C.Structure):
+    """Mirror of `struct FtaRotaryParams` (include/fta.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("q_sb", _i64), ("q_sh", _i64), ("q_sq", _i64),
+        ("k", _vp), ("k_sb", _i64), ("k_sh", _i64), ("k_sq", _i64),
+        ("v", _vp), ("v_sb", _i64), ("v_sh", _i64), ("v_sq", _i64),
+        ("q_out", _vp), ("k_out", _vp),
+        ("k_cache", _vp), ("kc_sb", _i64), ("kc_sh", _i64), ("kc_st", _i64),
+        ("v_cache", _vp), ("vc_sb", _i64), ("vc_sh", _i64), ("vc_st", _i64),
+        ("kv_seq_len", _vp), ("block_table", _vp), ("bt_sb", _i64),
+        ("positions", _vp), ("pos_sb", _i64), ("pos_sq", _i64), ("offsets", _vp), ("inv_freq", _vp),
+        ("amplitude", _f32), ("layout", _i32), ("inverse", _i32), ("n_freq", _i32), ("len_is_i64", _i32), ("pos_is_i64", _i32),
+        ("B", _i32), ("H", _i32), ("Hkv", _i32), ("Q", _i32), ("D", _i32), ("ctx", _i32),
+        ("page_size", _i32), ("n_pages", _i32), ("dtype", _i32), ("reserved_", _i32),
+    ]
+
+
+class FtaEvictParams(C.Structure):
+    """Mirror of `struct FtaEvictParams` (include/fta.h)."""
+
+    _fields_ = [
+        ("k_cache", _vp), ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64),
+        ("v_cache", _vp), ("v_sb", _i64), ("v_sh", _i64), ("v_st", _i64),
+        ("kv_seq_len", _vp), ("block_table", _vp), ("bt_sb", _i64), ("row_weights", _vp), ("rw_sb", _i64), ("rw_sh", _i64), ("kept", _vp),
+        ("len_is_i64", _i32), ("B", _i32), ("Hkv", _i32), ("D", _i32), ("ctx", _i32), ("page_size", _i32), ("n_pages", _i32),
+        ("budget", _i32), ("recent", _i32), ("reserved_", _i32),
+    ]
+
+
+class FtaLogprobParams(C.Structure):
+    """Mirror of `struct FtaLogprobParams` (include/fta.h)."""
+
+    _fields_ = [
+        ("logits", _vp), ("l_sr", _i64), ("tokens", _vp), ("t_sr", _i64),
+        ("logprobs", _vp), ("entropy", _vp), ("lse", _vp), ("top_logprobs", _vp), ("top_ids", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+        ("rows", _i32), ("vocab", _i32), ("n_tokens", _i32), ("top_k", _i32), ("dtype", _i32), ("tokens_are_i64", _i32),
+    ]
+
+
 def _packer(cls):
     """The fields of one call as the bytes of the C struct, in one step: filling a ctypes structure
     field by field costs several times as much, and a decoding step makes many small calls."""
     code = {_vp: "P", _i64: "q", _i32: "i", _f32: "f"}
-    fmt = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    fmt = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0q")  # padded to the struct's alignment
     assert fmt.size == C.sizeof(cls)
     return fmt.pack
 
 
 pack_token = _packer(FtaTokenParams)
+pack_rotary = _packer(FtaRotaryParams)
+pack_evict = _packer(FtaEvictParams)
+pack_logprob = _packer(FtaLogprobParams)
 
 # every symbol include/fta.h declares: (restype, argtypes)
 SYMBOLS = {
@@ -143,6 +187,11 @@ SYMBOLS = {
     "fta_merge_parts": (C.c_int, [C.POINTER(FtaMergeParams), _vp]),
     "fta_decode_token_workspace_bytes": (_i64, [_vp]),
     "fta_decode_token": (C.c_int, [_vp, _vp]),
+    "fta_apply_rotary": (C.c_int, [_vp, _vp]),
+    "fta_append_tokens": (C.c_int, [_vp, _vp]),
+    "fta_evict_rows": (C.c_int, [_vp, _vp]),
+    "fta_token_logprobs_workspace_bytes": (_i64, [_vp]),
+    "fta_token_logprobs": (C.c_int, [_vp, _vp]),
     "fta_commit_accepted": (C.c_int, [C.POINTER(FtaCommitParams), _vp]),
     "fta_exchange_merge": (C.c_int, [C.POINTER(FtaExchangeParams), _vp]),
     "fta_plan_host": (_i64, [C.POINTER(FtaParams), C.POINTER(_i64), C.POINTER(_i64), _i64,

@@ -27,6 +27,9 @@ SOURCES = [
     "fta_stage1_mma_d64.cu",
     "fta_stage1_mma_d128.cu",
     "fta_stage1_mma_d256.cu",
+    "fta_rotary.cu",
+    "fta_evict.cu",
+    "fta_logprobs.cu",
     "fta_token_join.cu",
     "fta_token_d32.cu",
     "fta_token_d64.cu",

@@ -1,4 +1,5 @@
-"""The decoding step without a draft tree: attention of one new token per sequence over the cache.
+"""The decoding step without a draft tree: attention of one new token per sequence over the cache,
+and the eviction of the rows that the attention looked at least.
 
 Shapes, strides, lengths and page tables are those of `flash_decoding_attention` and
 `flash_decoding_attention_paged` with q_len = 1; the new token's own key and value are already in
@@ -75,8 +76,8 @@ def _decode(q, k, v, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv
     rw, rw_sb, rw_sh = 0, 0, 0
     if row_weights is not None:
         assert row_weights.dtype == torch.float32 and row_weights.dim() == 3 and row_weights.device == dev \
-            and row_weights.size(0) == B and row_weights.size(1) == Hkv and row_weights.size(2) >= ctx and row_weights.stride(2) == 1, \
-            "row_weights must be [bsz, num_kv_heads, ctx] fp32 on q's device, unit stride along ctx"
+            and row_weights.size(0) == B and row_weights.size(1) == Hkv and row_weights.size(2) >= ctx and row_weights.stride(2) == 1 \
+            and not _overlaps(row_weights), "row_weights must be [bsz, num_kv_heads, ctx] fp32 on q's device, unit stride along ctx"
         rw, rw_sb, rw_sh = row_weights.data_ptr(), row_weights.stride(0), row_weights.stride(1)
     out = torch.empty((B, H, 1, D), dtype=dt, device=dev)
     lse = torch.empty((B, H, 1), dtype=torch.float32, device=dev) if return_lse else None
@@ -156,3 +157,62 @@ def decode_attention_paged(q, k_pages, v_pages, block_table, kv_seq_len, *, max_
     """
     return _decode(q, k_pages, v_pages, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv_group_num, softcap, alibi_slopes, window,
                    row_weights, return_lse)
+
+
+def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: int, *, block_table: Optional[torch.Tensor] = None):
+    """Bring every sequence longer than `budget` rows back to it, in place, per KV head.
+
+    Kept are the last `recent` rows and, of the others, the budget - recent with the largest
+    row_weights (ties: the lower row; NaN counts as largest).  They close up to rows [0, budget) in
+    their old order and their weights move with them.
+
+    Args:
+        k_cache, v_cache: dense [bsz, num_kv_heads, ctx, head_dim], or pools of pages with
+            `block_table`, updated in place; rows at or past the new length keep what they held.
+            No page may belong to two sequences: moving one's rows would change the other's.
+        kv_seq_len: [bsz] int32/int64 on the device, becomes min(length, budget) in place.
+        row_weights: [bsz, num_kv_heads, ctx] fp32 as decode_attention adds them up, updated in place:
+            0 from the new length to the old one, so that appended rows start at 0.
+        budget, recent: 1 <= budget, 0 <= recent <= budget.
+
+    Returns kept [bsz, num_kv_heads, budget] int32, the old row of every row now in the cache (-1 past
+    a shorter sequence's end).  Keys keep the rotary positions they were written with; a caller that
+    needs rows' positions keeps them by `kept`.  Asynchronous on the current stream of the caches'
+    device, no host synchronisation.
+    """
+    lib = _lib.load()
+    if not k_cache.is_cuda:
+        raise RuntimeError("evict_rows runs on CUDA tensors only (no CPU path exists)")
+    dt, dev = k_cache.dtype, k_cache.device
+    assert dt in _DT and k_cache.dim() == 4, "caches must be fp16 or bf16 [.., num_kv_heads, rows, head_dim]"
+    B, Hkv, D = kv_seq_len.size(0) if kv_seq_len.dim() == 1 else -1, k_cache.size(1), k_cache.size(3)
+    assert D in (32, 64, 128, 256)
+    ctx = _check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
+    _check_lengths(kv_seq_len, B, dev)
+    assert rows_ok(k_cache) and rows_ok(v_cache) and not _overlaps(k_cache) and not _overlaps(v_cache), \
+        "caches are updated in place: they must have 16-byte rows and must not be expanded"
+    assert B <= 1 or kv_seq_len.stride(0) == 1, "kv_seq_len is updated in place and must be contiguous"
+    assert row_weights.dtype == torch.float32 and row_weights.dim() == 3 and row_weights.device == dev and row_weights.size(0) == B \
+        and row_weights.size(1) == Hkv and row_weights.size(2) >= ctx and row_weights.stride(2) == 1 and not _overlaps(row_weights), \
+        "row_weights must be [bsz, num_kv_heads, ctx] fp32 on the caches' device, unit stride along ctx"
+    budget, recent = int(budget), int(recent)
+    assert 1 <= budget <= 0x7fffffff and 0 <= recent <= budget, "1 <= budget and 0 <= recent <= budget"
+    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
+    if B == 0:
+        return kept
+    ks, vs = k_cache.stride(), v_cache.stride()
+    paged = block_table is not None
+    p = _lib.pack_evict(
+        k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2], kv_seq_len.data_ptr(),
+        block_table.data_ptr() if paged else 0, block_table.stride(0) if paged else 0,
+        row_weights.data_ptr(), row_weights.stride(0), row_weights.stride(1), kept.data_ptr(),
+        1 if kv_seq_len.dtype == torch.int64 else 0, B, Hkv, D, ctx, k_cache.size(2) if paged else 0, k_cache.size(0) if paged else 0,
+        budget, recent, 0)
+    with on_device(dev) as stream:
+        _lib.check(lib.fta_evict_rows(p, stream), "fta_evict_rows")
+    return kept
+
+
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether some dimension of an in-place argument is broadcast (stride 0)."""
+    return any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))

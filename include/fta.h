@@ -292,6 +292,115 @@ typedef struct FtaTokenParams {
 int64_t fta_decode_token_workspace_bytes(const FtaTokenParams* p);
 int fta_decode_token(const FtaTokenParams* p, void* stream);
 
+/*
+ * Rotary positions, and the append of new tokens to the cache.  No counterpart in the reference.
+ * Pair i < n_freq of a head's first 2 * n_freq elements turns by angle = position * inv_freq[i]:
+ *   (x1, x2) -> amplitude * (x1 cos - x2 sin, x2 cos + x1 sin)
+ * where the pair is elements (i, i + n_freq) (FTA_ROTARY_HALF) or (2 i, 2 i + 1)
+ * (FTA_ROTARY_INTERLEAVED); the other elements are copied.  inverse turns back by the same angles
+ * (times the same amplitude): the transpose, and so the gradient.
+ *   position of token i of sequence b = positions[b * pos_sb + i * pos_sq] + offset, where offset is
+ *   offsets[i], or, without offsets, i if pos_sq is 0 and 0 otherwise.
+ * fta_apply_rotary: q, k -> q_out, k_out (k may be NULL with Hkv = 0).  v and the cache are not used.
+ * fta_append_tokens: q -> q_out as above; rotated k and v as it is become cache rows kv_seq_len[b] + i;
+ *   rows at or past ctx and rows of pages outside [0, n_pages) are dropped; kv_seq_len[b] grows by Q
+ *   in place, at most to ctx.  positions NULL: kv_seq_len[b] before the call.  n_freq 0 turns nothing;
+ *   q may then be NULL with H = 0.
+ * inv_freq is [n_freq] float64, finite.  An angle is position * (inv_freq / 2 pi) modulo one turn, exact
+ * but for the quotient's rounding in 64 bits, then rounded to 2^-32 of a turn.
+ */
+#define FTA_ROTARY_HALF 0
+#define FTA_ROTARY_INTERLEAVED 1
+typedef struct FtaRotaryParams {
+  const void* q; /* [B, H, Q, D] */
+  int64_t q_sb, q_sh, q_sq;
+  const void* k; /* [B, Hkv, Q, D] */
+  int64_t k_sb, k_sh, k_sq;
+  const void* v;
+  int64_t v_sb, v_sh, v_sq;
+  void* q_out; /* contiguous [B, H, Q, D] */
+  void* k_out; /* contiguous [B, Hkv, Q, D] */
+  void* k_cache;
+  int64_t kc_sb, kc_sh, kc_st;
+  void* v_cache;
+  int64_t vc_sb, vc_sh, vc_st;
+  void* kv_seq_len;
+  const int32_t* block_table;
+  int64_t bt_sb;
+  const void* positions;
+  int64_t pos_sb, pos_sq;
+  const int32_t* offsets; /* optional [Q] */
+  const double* inv_freq;
+  float amplitude;
+  int32_t layout, inverse;
+  int32_t n_freq;
+  int32_t len_is_i64, pos_is_i64;
+  int32_t B, H, Hkv, Q, D, ctx;
+  int32_t page_size, n_pages;
+  int32_t dtype;
+  int32_t reserved_;
+} FtaRotaryParams;
+
+int fta_apply_rotary(const FtaRotaryParams* p, void* stream);
+int fta_append_tokens(const FtaRotaryParams* p, void* stream);
+
+/*
+ * Eviction: brings every sequence longer than `budget` rows back to it, in place, per KV head.
+ * Kept are its last `recent` rows and, of the others, the budget - recent with the largest
+ * row_weights (ties: the lower row; NaN counts as largest); they move up to rows [0, budget) in their
+ * old order, and their weights with them.  row_weights of rows [budget, L) become 0, K and V there
+ * stay as they are.  kv_seq_len[b] becomes min(L, budget).  Other sequences are left alone.
+ *   kept  [B, Hkv, budget] int32, contiguous: the old row of every new row, -1 past a sequence's end
+ * A page outside [0, n_pages) is neither read nor written.
+ */
+typedef struct FtaEvictParams {
+  void* k_cache;
+  int64_t k_sb, k_sh, k_st;
+  void* v_cache;
+  int64_t v_sb, v_sh, v_st;
+  void* kv_seq_len;
+  const int32_t* block_table;
+  int64_t bt_sb;
+  float* row_weights; /* [B, Hkv, ctx] */
+  int64_t rw_sb, rw_sh;
+  int32_t* kept;
+  int32_t len_is_i64;
+  int32_t B, Hkv, D, ctx;
+  int32_t page_size, n_pages;
+  int32_t budget, recent;
+  int32_t reserved_;
+} FtaEvictParams;
+
+int fta_evict_rows(const FtaEvictParams* p, void* stream);
+
+/*
+ * Log probabilities of given tokens under rows of logits, with the rows' log-sum-exp, entropy and
+ * top_k likeliest tokens.  All natural logs in fp32.  Rows whose logits are all -inf: lse = -inf,
+ * entropy = 0, every log probability -inf.  A token outside [0, vocab) gets -inf.  Ties among the top
+ * go to the lower token; a NaN logit makes lse, entropy and log probabilities NaN and ranks first.
+ */
+#define FTA_MAX_TOP_K 64
+typedef struct FtaLogprobParams {
+  const void* logits; /* [rows, vocab], unit stride along the vocabulary */
+  int64_t l_sr;
+  const void* tokens; /* [rows, n_tokens], optional */
+  int64_t t_sr;
+  float* logprobs;     /* [rows, n_tokens] contiguous */
+  float* entropy;      /* [rows] */
+  float* lse;          /* [rows] */
+  float* top_logprobs; /* [rows, top_k] contiguous */
+  int64_t* top_ids;    /* [rows, top_k] contiguous */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t rows, vocab, n_tokens, top_k;
+  int32_t dtype; /* FTA_DTYPE_* */
+  int32_t tokens_are_i64;
+} FtaLogprobParams;
+
+/* Bytes of workspace the call needs; negative: -FTA_E_*.  rows, vocab, top_k and dtype are read. */
+int64_t fta_token_logprobs_workspace_bytes(const FtaLogprobParams* p);
+int fta_token_logprobs(const FtaLogprobParams* p, void* stream);
+
 /* Text for an FTA_E_* code.  No counterpart in the reference (it raises AssertionError,
    flash_tree_attn.py:263-291). */
 const char* fta_strerror(int code);
