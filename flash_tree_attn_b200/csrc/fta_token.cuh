@@ -8,12 +8,14 @@
 // operations, 2 * G operations a byte: the cache stream (HBM) is the floor at any G <= 16.
 //
 // Layout.  A group's heads (8 or 16, padded) are the N side of mma.m16n8k16 and 16 cache rows its M
-// side: S^T = K q^T, O^T = V^T P^T.  A contraction does not care for the order of its terms, so each
-// lane takes 16 contiguous bytes of a K row as its part of two k-steps, and of V it takes 16 bytes of
-// four rows, from which byte permutes make the pairs along the rows that the product wants.  So a lane
-// reads from shared memory exactly the bytes it copied there itself: the ring is private to the lane,
-// there is no barrier and no bank conflict in the loop, and each warp walks its own rows (16 of every
-// 64-row tile) at its own pace.  The warps meet once per piece, to join their (m, l, O).
+// side: S^T = K q^T, O^T = V^T P^T.  A contraction does not care for the order of its terms, so a lane
+// takes 16 contiguous bytes of a K row as its part of two k-steps, and of V it takes 16 bytes of four
+// rows, from which byte permutes make the pairs along the rows that the product wants.  Each warp copies
+// and multiplies its own rows (16 of every 64-row tile) through a ring of its own, so no barrier but the
+// warp's stands in the loop.  The warps meet once per piece, to join their (m, l, O).
+//
+// Measured: 64 ragged sequences of up to 8192 rows (32/8 heads of 128, pages of 64 rows, 1.1 GB of K and
+// V): 178 us, 6.2 TB/s, 95 % of the measured copy rate.
 #pragma once
 #include "fta_common.cuh"
 

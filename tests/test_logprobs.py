@@ -68,7 +68,7 @@ def test_rows_that_start_anywhere(dtype, shift):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["equal", "two values", "masked", "all masked", "nan", "inf", "rising", "one high", "far"])
+@pytest.mark.parametrize("kind", ["equal", "two values", "masked", "all masked", "nan", "inf", "rising", "one high", "far", "lowest", "lowest and masked"])
 @pytest.mark.parametrize("V", [50, 3000, 70001])
 def test_rows_that_tie_or_are_masked(kind, V):
     import flash_tree_attn_b200 as fta
@@ -98,7 +98,15 @@ def test_rows_that_tie_or_are_masked(kind, V):
         x[:, 3] = 300.0
     elif kind == "far":
         x = x - 20000.0
-    for dtype in (torch.float32, torch.bfloat16):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        if kind.startswith("lowest"):  # masked with the type's lowest value, and two rows of nothing else
+            x = torch.randn(4, V, generator=g)
+            x[:2] = torch.finfo(dtype).min
+            x[2, 1:] = torch.finfo(dtype).min
+            if kind.endswith("masked"):
+                x[1:, ::3] = float("-inf")
+        if dtype == torch.float16 and kind == "far":
+            x = x / 4
         y = x.to(dtype).cuda()
         t = _tokens(4, V, 2, g)
         _check(y, t, 40, fta.token_logprobs(y, t, 40))
