@@ -154,7 +154,7 @@ class FtaLogprobParams(C.Structure):
 
     _fields_ = [
         ("logits", _vp), ("l_sr", _i64), ("tokens", _vp), ("t_sr", _i64),
-        ("logprobs", _vp), ("entropy", _vp), ("lse", _vp), ("top_logprobs", _vp), ("top_ids", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+        ("logprobs", _vp), ("entropy", _vp), ("lse", _vp), ("top_logprobs", _vp), ("top_ids", _vp),
         ("rows", _i32), ("vocab", _i32), ("n_tokens", _i32), ("top_k", _i32), ("dtype", _i32), ("tokens_are_i64", _i32),
     ]
 
@@ -190,7 +190,6 @@ SYMBOLS = {
     "fta_apply_rotary": (C.c_int, [_vp, _vp]),
     "fta_append_tokens": (C.c_int, [_vp, _vp]),
     "fta_evict_rows": (C.c_int, [_vp, _vp]),
-    "fta_token_logprobs_workspace_bytes": (_i64, [_vp]),
     "fta_token_logprobs": (C.c_int, [_vp, _vp]),
     "fta_commit_accepted": (C.c_int, [C.POINTER(FtaCommitParams), _vp]),
     "fta_exchange_merge": (C.c_int, [C.POINTER(FtaExchangeParams), _vp]),
@@ -244,27 +243,25 @@ def check(code: int, where: str) -> None:
         raise FtaError(code, where)
 
 
-def rows_ok(t) -> bool:
-    """Whether the rows of a 4-D tensor can be copied in 16-byte pieces (16-bit elements)."""
+def rows_of(t):
+    """(data pointer, strides of the three leading dimensions) of a 4-D tensor whose rows can be copied in
+    16-byte pieces (16-bit elements), None of another."""
     a, b, c, d = t.stride()
-    return d == 1 and not (a | b | c) & 7 and not t.data_ptr() & 15
+    ptr = t.data_ptr()
+    return None if d != 1 or (a | b | c) & 7 or ptr & 15 else (ptr, a, b, c)
 
 
-class on_device:
-    """The current stream of a tensor's device, that device made current for the block if it is not."""
+_current_device = torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, dev):
-        self.index = dev.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-        return False
+def launch(fn, p, index: int, where: str) -> None:
+    """Call a C entry with the packed parameters on the current stream of device `index`, that device
+    made current if it is not."""
+    if _current_device() == index:
+        code = fn(p, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(p, _raw_stream(index))
+    if code:
+        raise FtaError(code, where)

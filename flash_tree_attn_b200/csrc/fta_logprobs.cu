@@ -14,14 +14,21 @@
 // memory, so there is room for about 10 instructions an element, and 16 exponentials a clock.  A row is
 // cut into pieces that a block holds in registers (8 chunks of 16 bytes a thread), so the maximum (packed,
 // per chunk), the sums (6 instructions an element) and the search for the likeliest need no second
-// read, and a few long rows spread over the machine.  A second kernel joins the pieces.
+// read.  A row's pieces are a cluster's blocks (a block takes several of a row with more than 8): they
+// spread a few long rows over the machine, and join through distributed shared memory, without a
+// workspace or a second kernel.
 //
 // The likeliest of a piece: every warp's q-th largest of its lanes' maxima is a bound that at least q
-// of the warp's elements reach; the least of those bounds over W warps is reached by q W >= k elements.
-// Only chunks whose maximum reaches it are looked at again (typically two or three times k elements
-// do), and what is found is ranked by counting.  Where too many do (ties, masked vocabularies) the exact
-// bound is found bit by bit instead.
+// of the warp's elements reach; the w-th largest of those bounds is reached by q w >= k elements.
+// Chunks whose maximum reaches it (typically less than twice k) are listed, their elements shared
+// out over the block, and those that reach it ranked by counting.  Looking at a chunk where it was found
+// would hold up its whole warp: a listed chunk costs a few instructions there.  Where too many reach the
+// bound (ties, masked vocabularies) the exact one is found bit by bit instead.
+#include <cooperative_groups.h>
+
 #include "fta_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -29,8 +36,9 @@ constexpr int kThreads = 256;     // 4 blocks an SM: one computes while the othe
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunks = 8;        // 16-byte chunks per thread
 constexpr int kListed = 1024;     // elements ranked by counting
+constexpr int kListedChunks = 256;
 constexpr int kMostRounds = 16;   // largest q; below 4 full warps a piece has fewer than kListed elements
-constexpr int kJoin = 128;
+constexpr int kMostBlocks = 8;    // of a cluster, so of a row
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
@@ -123,7 +131,7 @@ __device__ __forceinline__ unsigned long long rank_key(uint32_t k, int token) {
   return ((unsigned long long)k << 32) | (uint32_t)(0xffffffffu - (uint32_t)token);
 }
 
-struct Piece { float m, s, t, unused; };
+struct Sums { float m, s, t; };  // s and t in log2 units relative to m
 
 template <int N> __device__ __forceinline__ int block_sum(int x, int* scratch) {
   x = __reduce_add_sync(0xffffffffu, x);
@@ -136,103 +144,150 @@ template <int N> __device__ __forceinline__ int block_sum(int x, int* scratch) {
   return sum;
 }
 
-// grid = rows * pieces.  Chunks lie on 16-byte boundaries of memory, whatever the row's start: element
-// e of the row is element e + head of the chunks.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_piece_kernel(const FtaLogprobParams p, const int pieces) {
-  constexpr int VE = Vec<T>::n;
-  static_assert(kThreads * kChunks * VE <= 1 << 15, "the search over a piece's tokens takes 16 steps");
-  __shared__ unsigned long long list[kListed];
-  __shared__ float s_a[kWarps], s_b[kWarps], s_c[kWarps];
-  __shared__ int s_i[kWarps];
-  __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long row = blockIdx.x / pieces;
-  const int piece = blockIdx.x - (int)row * pieces;
-  const T* x = reinterpret_cast<const T*>(p.logits) + row * p.l_sr;
-  const int head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int base = piece * (kThreads * kChunks);  // first chunk of the piece
-  const int k = p.top_k;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join's blocks wait for this grid's end
-
-  uint4 raw[kChunks];
+// how many of keys[0, n) are larger; the array is zeroed up to a multiple of 8 (the loads of 8 go out
+// together: a loop that waits for each of them is most of the time of a small row)
+__device__ __forceinline__ int larger(const unsigned long long* keys, int n, unsigned long long own) {
+  int before = 0;
+  for (int j = 0; j < n; j += 8) {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int e0 = (base + c * kThreads + tid) * VE - head;
-    if (e0 >= 0 && e0 + VE <= p.vocab) {
-      raw[c] = __ldcs(reinterpret_cast<const uint4*>(x + e0));
-    } else {  // the row's ends
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const uint32_t v = e0 + i >= 0 && e0 + i < p.vocab ? Vec<T>::bits(x + e0 + i) : Vec<T>::kLowest;
-        w[i * 4 / VE] |= v << (VE == 8 ? 16 * (i & 1) : 0);
-      }
-      raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int u = 0; u < 8; u += 2) {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(keys + j + u);
+      before += (x.x > own) + (x.y > own);
     }
   }
-  float top[kChunks], mine = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    top[c] = Vec<T>::max(raw[c]);
-    mine = fmaxf(mine, top[c]);
-  }
-  float m = mine;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return before;
+}
 
-  // the warp's bound: its q-th largest lane maximum
-  const int chunks = min(kThreads * kChunks, fta_cdiv(p.vocab + head, VE) - base);  // of this piece
-  const int full = min(kWarps, (chunks - (head > 0 && piece == 0 ? 1 : 0)) / 32);    // warps whose lanes all hold elements
-  float bound = -INFINITY;
-  if (k > 0 && full > 0 && fta_cdiv(k, full) <= kMostRounds) {
-    const int q = fta_cdiv(k, full);
-    uint32_t key = ordered(mine);
-    if (warp < full) {
-      uint32_t kth = 0;
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+  if (b.s == 0.f) return a;  // nothing but -inf
+  if (a.s == 0.f) return b;
+  const float m = fmaxf(a.m, b.m);
+  const float da = (a.m - m) * FTA_LOG2E, db = (b.m - m) * FTA_LOG2E, fa = fta_exp2(da), fb = fta_exp2(db);
+  return Sums{m, fa * a.s + fb * b.s, (fa == 0.f ? 0.f : fa * (a.t + da * a.s)) + (fb == 0.f ? 0.f : fb * (b.t + db * b.s))};
+}
+
+// grid = rows * (blocks of a cluster); block i of a row takes its pieces [i * rounds, (i + 1) * rounds).
+// Chunks lie on 16-byte boundaries of memory, whatever the row's start: element e of the row is element
+// e + head of the chunks.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobParams p, const int blocks, const int rounds) {
+  constexpr int VE = Vec<T>::n;
+  static_assert(kThreads * kChunks * VE <= 1 << 15, "the search over a piece's tokens takes 16 steps");
+  __shared__ __align__(16) unsigned long long list[kListed + FTA_MAX_TOP_K + 8];
+  __shared__ unsigned long long best[FTA_MAX_TOP_K];  // the likeliest so far, in order; 0: none
+  __shared__ Sums s_sums;
+  __shared__ float s_a[kWarps], s_b[kWarps], s_c[kWarps];
+  __shared__ int s_i[kWarps];
+  __shared__ uint32_t s_key[kWarps];
+  __shared__ int s_n, s_listed;
+  __shared__ uint4 s_chunk[kListedChunks];
+  __shared__ int s_where[kListedChunks];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long row = blockIdx.x / blocks;
+  const int block = blockIdx.x - (int)row * blocks;
+  const T* x = reinterpret_cast<const T*>(p.logits) + row * p.l_sr;
+  const int head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int k = p.top_k;
+  Sums sums = {-INFINITY, 0.f, 0.f};
+  if (tid < k) best[tid] = 0;
+  // the first block of a row answers for its tokens; their logits are asked for before all else
+  auto logit_of = [&](int i, bool& inside) {
+    const long long tok = p.tokens_are_i64 ? reinterpret_cast<const long long*>(p.tokens)[row * p.t_sr + i]
+                                           : (long long)reinterpret_cast<const int*>(p.tokens)[row * p.t_sr + i];
+    inside = tok >= 0 && tok < p.vocab;
+    return inside ? to_float(x[tok]) : -INFINITY;
+  };
+  bool asked_inside = false;
+  const float asked = block == 0 && tid < p.n_tokens ? logit_of(tid, asked_inside) : 0.f;
+
+  for (int round = 0; round < rounds; ++round) {
+    const int base = (block * rounds + round) * (kThreads * kChunks);  // first chunk of the piece
+    const int chunks = min(kThreads * kChunks, fta_cdiv(p.vocab + head, VE) - base);
+    if (chunks <= 0) break;
+    __syncthreads();  // the round before is done with the shared arrays
+    uint4 raw[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int e0 = (base + c * kThreads + tid) * VE - head;
+      if (e0 >= 0 && e0 + VE <= p.vocab) {
+        raw[c] = __ldcs(reinterpret_cast<const uint4*>(x + e0));
+      } else {  // the row's ends
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const uint32_t v = e0 + i >= 0 && e0 + i < p.vocab ? Vec<T>::bits(x + e0 + i) : Vec<T>::kLowest;
+          w[i * 4 / VE] |= v << (VE == 8 ? 16 * (i & 1) : 0);
+        }
+        raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    float top[kChunks], mine = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      top[c] = Vec<T>::max(raw[c]);
+      mine = fmaxf(mine, top[c]);
+    }
+    float m = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+
+    // the warp's bound: its q-th largest lane maximum
+    const int full = min(kWarps, chunks / 32);   // warps whose lanes all hold elements
+    const int q = full > 0 ? fta_cdiv(k, full) : kMostRounds + 1;
+    const bool bounded = k > 0 && q <= kMostRounds;
+    uint32_t kth = 0;
+    if (bounded && warp < full) {
+      uint32_t key = ordered(mine);
       for (int i = 0; i < q; ++i) {
         kth = __reduce_max_sync(0xffffffffu, key);
         const unsigned who = __ballot_sync(0xffffffffu, key == kth);
         if (lane == __ffs(who) - 1) key = 0;
       }
-      bound = unordered(kth);
-    } else {
-      bound = INFINITY;
     }
-  }
-  if (lane == 0) { s_a[warp] = m; s_b[warp] = bound; }
-  if (tid == 0) s_n = 0;
-  __syncthreads();
-  m = -INFINITY;
-  bound = INFINITY;
+    if (lane == 0) { s_a[warp] = m; s_key[warp] = kth; }
+    if (tid == 0) s_n = s_listed = 0;
+    __syncthreads();
+    m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) { m = fmaxf(m, s_a[w]); bound = fminf(bound, s_b[w]); }
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_a[w]);
+    float bound = -INFINITY;
+    if (bounded) {  // the w-th largest of the warps' bounds: the one that w - 1 others come before
+      kth = s_key[lane % kWarps];
+      int before = 0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const uint32_t o = __shfl_sync(0xffffffffu, kth, i);
+        before += o > kth || (o == kth && i < lane % kWarps);
+      }
+      const unsigned who = __ballot_sync(0xffffffffu, before == fta_cdiv(k, q) - 1);
+      bound = unordered(__shfl_sync(0xffffffffu, kth, __ffs(who) - 1));
+    }
+    // what came in earlier rounds need not be reached again; a NaN there stays out of the comparison
+    if (k > 0 && best[k - 1] != 0) bound = fmaxf(bound, unordered((uint32_t)(best[k - 1] >> 32)));
 
-  const bool near = fabsf(m) < 30000.f;
-  const float m2 = __fmul_rn(m, FTA_LOG2E), safe = m == -INFINITY ? 0.f : m;
-  float s = 0.f, t = 0.f;
-  if (near) {
+    const bool near = fabsf(m) < 30000.f;
+    const float m2 = __fmul_rn(m, FTA_LOG2E), safe = m == -INFINITY ? 0.f : m;
+    float s = 0.f, t = 0.f;
+    if (near) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      if (c * kThreads < chunks) Vec<T>::add(raw[c], m2, s, t);
-  } else {
+      for (int c = 0; c < kChunks; ++c)
+        if (c * kThreads < chunks) Vec<T>::add(raw[c], m2, s, t);
+    } else {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+      for (int c = 0; c < kChunks; ++c) {
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
-      for (int i = 0; i < VE; ++i) add_exp(max_nan((Vec<T>::get(w[i * 4 / VE], i & 1) - safe) * FTA_LOG2E, -1e30f), s, t);
+        for (int i = 0; i < VE; ++i) add_exp(max_nan((Vec<T>::get(w[i * 4 / VE], i & 1) - safe) * FTA_LOG2E, -1e30f), s, t);
+      }
     }
-  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    t += __shfl_xor_sync(0xffffffffu, t, o);
-  }
-  __syncthreads();
-  if (lane == 0) { s_b[warp] = s; s_c[warp] = t; }
-  __syncthreads();
-  uint8_t* ws = reinterpret_cast<uint8_t*>(p.workspace);
-  if (tid == 0) {
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    __syncthreads();
+    if (lane == 0) { s_b[warp] = s; s_c[warp] = t; }
+    __syncthreads();
     s = t = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) { s += s_b[w]; t += s_c[w]; }
@@ -241,111 +296,113 @@ __global__ void __launch_bounds__(kThreads) logprob_piece_kernel(const FtaLogpro
       t = f * (t - r * s);
       s *= f;
     }
-    reinterpret_cast<Piece*>(ws)[row * pieces + piece] = Piece{m, s, t, 0.f};
-  }
-  if (k == 0) return;
+    sums = join(sums, Sums{m, s, t});
+    if (k == 0) continue;
 
-  // list what reaches the bound (NaN does): the few chunks that do are read again, from the cache
+    // list the chunks that reach the bound (NaN does), then their elements
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    if (top[c] < bound || c * kThreads >= chunks) continue;
-    const int tok0 = (base + c * kThreads + tid) * VE - head;
-    for (int i = max(0, -tok0); i < VE && tok0 + i < p.vocab; ++i) {
-      const float v = to_float(x[tok0 + i]);
-      if (v < bound) continue;
+    for (int c = 0; c < kChunks; ++c) {
+      if (top[c] < bound || c * kThreads + tid >= chunks) continue;
       const int at = atomicAdd(&s_n, 1);
-      if (at < kListed) list[at] = rank_key(ordered(v), tok0 + i);
+      if (at < kListedChunks) {
+        s_chunk[at] = raw[c];
+        s_where[at] = c * kThreads + tid;
+      }
     }
-  }
-  __syncthreads();
-  int n = s_n;
-  if (n > kListed) {
-    const int lo = max(0, base * VE - head), hi = min(p.vocab, (base + kThreads * kChunks) * VE - head);
-    // The k-th largest value, bit by bit from the top: the largest key that at least k elements reach.
-    uint32_t key = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t at_least = key | (1u << bit);
-      int count = 0;
-      for (int i = lo + tid; i < hi; i += kThreads) count += ordered(to_float(x[i])) >= at_least;
-      if (block_sum<kWarps>(count, s_i) >= k) key = at_least;
+    __syncthreads();
+    const int reached = s_n;
+    for (int i = tid; i < min(reached, kListedChunks) * VE; i += kThreads) {
+      const int at = i / VE, e = i % VE;
+      const float v = Vec<T>::get(reinterpret_cast<const uint32_t*>(&s_chunk[at])[e * 4 / VE], e & 1);
+      const int tok = (base + s_where[at]) * VE - head + e;
+      if (v < bound || tok < 0 || tok >= p.vocab) continue;
+      const int to = atomicAdd(&s_listed, 1);
+      if (to < kListed) list[to] = rank_key(ordered(v), tok);
     }
-    // Of the elements equal to it the lowest tokens are wanted: those below the least `end` that makes k.
-    int end = lo;
-    for (int step = 1 << 15; step > 0; step >>= 1) {  // a piece holds at most 2^15 elements
-      int count = 0;
+    __syncthreads();
+    int n = s_listed;
+    if (reached > kListedChunks || n > kListed) {
+      const int lo = max(0, base * VE - head), hi = min(p.vocab, (base + kThreads * kChunks) * VE - head);
+      // The k-th largest value, bit by bit from the top: the largest key that at least k elements reach.
+      uint32_t key = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t at_least = key | (1u << bit);
+        int count = 0;
+        for (int i = lo + tid; i < hi; i += kThreads) count += ordered(to_float(x[i])) >= at_least;
+        if (block_sum<kWarps>(count, s_i) >= k) key = at_least;
+      }
+      // Of the elements equal to it the lowest tokens are wanted: those below the least `end` that makes k.
+      int end = lo;
+      for (int step = 1 << 15; step > 0; step >>= 1) {  // a piece holds at most 2^15 elements
+        int count = 0;
+        for (int i = lo + tid; i < hi; i += kThreads) {
+          const uint32_t o = ordered(to_float(x[i]));
+          count += o > key || (o == key && i < end + step);
+        }
+        if (block_sum<kWarps>(count, s_i) < k) end += step;
+      }
+      if (tid == 0) s_n = 0;
+      __syncthreads();
       for (int i = lo + tid; i < hi; i += kThreads) {
         const uint32_t o = ordered(to_float(x[i]));
-        count += o > key || (o == key && i < end + step);
+        if (o > key || (o == key && i <= end)) list[atomicAdd(&s_n, 1)] = rank_key(o, i);
       }
-      if (block_sum<kWarps>(count, s_i) < k) end += step;
+      __syncthreads();
+      n = s_n;
     }
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += kThreads) {
-      const uint32_t o = ordered(to_float(x[i]));
-      if (o > key || (o == key && i <= end)) list[atomicAdd(&s_n, 1)] = rank_key(o, i);
+    if (round > 0) {
+      for (int i = tid; i < k; i += kThreads) list[n + i] = best[i];
+      n += k;
     }
+    if (tid < 8) list[n + tid] = 0;
     __syncthreads();
-    n = s_n;
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long own = list[i];
+      const int before = larger(list, n, own);
+      if (before < k && own != 0) best[before] = own;
+    }
   }
-  unsigned long long* out = reinterpret_cast<unsigned long long*>(ws + (long long)p.rows * pieces * sizeof(Piece)) + (row * pieces + piece) * k;
-  for (int i = tid; i < n; i += kThreads) {
-    const unsigned long long own = list[i];
-    int before = 0;
-    for (int j = 0; j < n; ++j) before += list[j] > own;
-    if (before < k) out[before] = own;
-  }
-  for (int i = n + tid; i < k; i += kThreads) out[i] = 0;  // a short last piece
-}
 
-// grid = rows: joins a row's pieces.
-template <typename T>
-__global__ void __launch_bounds__(kJoin) logprob_join_kernel(const FtaLogprobParams p, const int pieces) {
-  extern __shared__ unsigned long long keys[];
-  const long long row = blockIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint8_t* ws = reinterpret_cast<const uint8_t*>(p.workspace);
-  const Piece* part = reinterpret_cast<const Piece*>(ws) + row * pieces;
-  float m = -INFINITY, s = 0.f, t = 0.f;
-  for (int i = 0; i < pieces; ++i) m = fmaxf(m, part[i].m);
-  for (int i = 0; i < pieces; ++i) {
-    const Piece q = part[i];
-    if (q.s == 0.f) continue;  // nothing but -inf
-    const float shift = (q.m - m) * FTA_LOG2E;
-    const float f = fta_exp2(shift);
-    s += f * q.s;
-    t += f == 0.f ? 0.f : f * (q.t + shift * q.s);
+  // the row's blocks join in the first one
+  cg::cluster_group cluster = cg::this_cluster();
+  if (blocks > 1) {
+    if (tid == 0) s_sums = sums;
+    cluster.sync();
+    if (block == 0) {
+      for (int i = 1; i < blocks; ++i) sums = join(sums, *cluster.map_shared_rank(&s_sums, i));
+      for (int i = tid; i < blocks * k; i += kThreads) list[i] = cluster.map_shared_rank(best, i / k)[i % k];
+      if (tid < 8) list[blocks * k + tid] = 0;
+    }
+    cluster.sync();  // the others' shared memory has been read: they may end
+    if (block != 0) return;
+  } else {
+    __syncthreads();
+    for (int i = tid; i < k; i += kThreads) list[i] = best[i];
+    if (tid < 8) list[k + tid] = 0;
+    __syncthreads();
   }
+  const float m = sums.m, s = sums.s;
   const float log2_s = fta_log2(s);
   const float log_s = log2_s * FTA_LN2;
-  const float lse = s == 0.f ? -INFINITY : m + log_s;
-  if (threadIdx.x == 0) {
-    p.lse[row] = lse;
-    p.entropy[row] = s == 0.f ? 0.f : (log2_s - t / s) * FTA_LN2;
+  if (tid == 0) {
+    p.lse[row] = s == 0.f ? -INFINITY : m + log_s;
+    p.entropy[row] = s == 0.f ? 0.f : (log2_s - sums.t / s) * FTA_LN2;
   }
   // (x - m) - log s: what m and lse have in common is not rounded
   auto log_p = [&](float v) { return s == 0.f || v == -INFINITY ? (s != s ? s : -INFINITY) : (v - m) - log_s; };
-  const T* x = reinterpret_cast<const T*>(p.logits) + row * p.l_sr;
-  for (int i = threadIdx.x; i < p.n_tokens; i += kJoin) {
-    const long long tok = p.tokens_are_i64 ? reinterpret_cast<const long long*>(p.tokens)[row * p.t_sr + i]
-                                           : (long long)reinterpret_cast<const int*>(p.tokens)[row * p.t_sr + i];
-    float lp = -INFINITY;
-    if (tok >= 0 && tok < p.vocab) lp = log_p(to_float(x[tok]));
-    p.logprobs[row * p.n_tokens + i] = lp;
+  for (int i = tid; i < p.n_tokens; i += kThreads) {
+    bool inside = asked_inside;
+    const float v = i == tid ? asked : logit_of(i, inside);
+    p.logprobs[row * p.n_tokens + i] = inside ? log_p(v) : -INFINITY;
   }
-  if (p.top_k == 0) return;
-  const int n = pieces * p.top_k;
-  const unsigned long long* in = reinterpret_cast<const unsigned long long*>(ws + (long long)p.rows * pieces * sizeof(Piece)) + row * n;
-  for (int i = threadIdx.x; i < n; i += kJoin) keys[i] = in[i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kJoin) {
-    const unsigned long long own = keys[i];
+  const int n = blocks * k;
+  for (int i = tid; i < n; i += kThreads) {
+    const unsigned long long own = list[i];
     if (own == 0) continue;
-    int before = 0;
-    for (int j = 0; j < n; ++j) before += keys[j] > own;
-    if (before < p.top_k) {
-      p.top_logprobs[row * p.top_k + before] = log_p(unordered((uint32_t)(own >> 32)));
-      p.top_ids[row * p.top_k + before] = (int64_t)(0xffffffffu - (uint32_t)own);
+    const int before = larger(list, n, own);
+    if (before < k) {
+      p.top_logprobs[row * k + before] = log_p(unordered((uint32_t)(own >> 32)));
+      p.top_ids[row * k + before] = (int64_t)(0xffffffffu - (uint32_t)own);
     }
   }
 }
@@ -356,46 +413,39 @@ int pieces_of(const FtaLogprobParams& p) {
   return fta_cdiv(p.vocab + ve - 1, kThreads * kChunks * ve);
 }
 
-int check_sizes(const FtaLogprobParams* p) {
-  if (!p || p->rows <= 0 || p->vocab <= 0 || p->top_k < 0 || p->top_k > p->vocab || p->n_tokens < 0) return FTA_E_BADARG;
-  if (p->dtype < FTA_DTYPE_F16 || p->dtype > FTA_DTYPE_F32) return FTA_E_BADARG;
-  if (p->top_k > FTA_MAX_TOP_K || p->vocab > (1 << 19)) return FTA_E_UNSUPPORTED;
-  if ((long long)p->rows * pieces_of(*p) > 0x7fffffffLL) return FTA_E_UNSUPPORTED;
-  return FTA_OK;
-}
-
-int64_t ws_bytes(const FtaLogprobParams& p) { return (int64_t)p.rows * pieces_of(p) * (sizeof(Piece) + 8 * p.top_k); }
-
 template <typename T>
 int run(const FtaLogprobParams& p, cudaStream_t st) {
   const int pieces = pieces_of(p);
-  logprob_piece_kernel<T><<<pieces * p.rows, kThreads, 0, st>>>(p, pieces);
-  const size_t smem = (size_t)pieces * p.top_k * 8;
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fta_cuda_fail(e);
+  // Blocks per row: enough to fill the machine, and no more.  A wave of blocks lasts as long as its
+  // rounds, and about one round more for the start and the end of a block, another one for a cluster's join.
+  const int slots = 148 * 4;
+  int blocks = 1, rounds = pieces;
+  long long least = 0x7fffffffffffffffLL;
+  for (int n = 1; n <= kMostBlocks && n <= pieces; ++n) {
+    const int r = fta_cdiv(pieces, n);
+    if (fta_cdiv(pieces, r) != n) continue;  // the last block would have nothing
+    const long long cost = (((long long)p.rows * n + slots - 1) / slots) * (r + (n > 1 ? 2 : 1));
+    if (cost < least) { least = cost; blocks = n; rounds = r; }
+  }
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows); cfg.blockDim = dim3(kJoin); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3(p.rows * blocks); cfg.blockDim = dim3(kThreads); cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, logprob_join_kernel<T>, p, pieces);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprob_kernel<T>, p, blocks, rounds);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
 
 }  // namespace
 
-extern "C" int64_t fta_token_logprobs_workspace_bytes(const FtaLogprobParams* p) {
-  if (int rc = check_sizes(p)) return -rc;
-  return ws_bytes(*p);
-}
-
 extern "C" int fta_token_logprobs(const FtaLogprobParams* p, void* stream) {
-  if (int rc = check_sizes(p)) return rc;
+  if (!p || p->rows <= 0 || p->vocab <= 0 || p->top_k < 0 || p->top_k > p->vocab || p->n_tokens < 0) return FTA_E_BADARG;
+  if (p->dtype < FTA_DTYPE_F16 || p->dtype > FTA_DTYPE_F32) return FTA_E_BADARG;
   if (!p->logits || !p->entropy || !p->lse || (p->n_tokens > 0 && (!p->tokens || !p->logprobs))) return FTA_E_BADARG;
   if (p->top_k > 0 && (!p->top_logprobs || !p->top_ids)) return FTA_E_BADARG;
   if (reinterpret_cast<uintptr_t>(p->logits) % (p->dtype == FTA_DTYPE_F32 ? 4 : 2) != 0) return FTA_E_BADARG;
-  if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 15) || p->workspace_bytes < ws_bytes(*p)) return FTA_E_WORKSPACE;
+  if (p->top_k > FTA_MAX_TOP_K || p->vocab > (1 << 21) || p->rows > (1 << 27)) return FTA_E_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
   if (p->dtype == FTA_DTYPE_F16) return run<__half>(*p, st);
   if (p->dtype == FTA_DTYPE_BF16) return run<__nv_bfloat16>(*p, st);

@@ -4,6 +4,8 @@ and the eviction of the rows that the attention looked at least.
 Shapes, strides, lengths and page tables are those of `flash_decoding_attention` and
 `flash_decoding_attention_paged` with q_len = 1; the new token's own key and value are already in
 the cache (see `append_tokens`).  All arithmetic happens in libfta.so.
+
+A decoding step makes many small calls, so the checks here read each tensor's attributes once.
 """
 from __future__ import annotations
 
@@ -13,30 +15,62 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import on_device, rows_ok
+from ._lib import launch, pack_evict, pack_token, rows_of
 
 _DT = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
-_LEN = (torch.int32, torch.int64)
+_LEN = {torch.int32: 0, torch.int64: 1}  # -> is int64
+_HEAD_DIMS = (32, 64, 128, 256)
+_f32 = torch.float32
 
 
-def _check_lengths(kv_seq_len: torch.Tensor, B: int, dev: torch.device) -> None:
-    assert kv_seq_len.dtype in _LEN and kv_seq_len.dim() == 1 and kv_seq_len.size(0) == B and kv_seq_len.device == dev, \
-        "kv_seq_len must be [bsz] int32 or int64 on q's device"
+def check_lengths(kv_seq_len: torch.Tensor, B: int, dev: int) -> int:
+    """1 for int64 lengths, 0 for int32 ones."""
+    is64 = _LEN.get(kv_seq_len.dtype)
+    assert is64 is not None and kv_seq_len.shape == (B,) and kv_seq_len.get_device() == dev, \
+        "kv_seq_len must be [bsz] int32 or int64 on the caches' device"
+    return is64
 
 
-def _check_caches(k: torch.Tensor, v: torch.Tensor, B: int, Hkv: int, D: int, dtype, dev, block_table: Optional[torch.Tensor]) -> int:
-    """The checks every entry makes of a dense or paged pair of caches; returns the rows that a sequence can hold."""
-    assert k.dtype == dtype and v.dtype == dtype, "cache dtype must equal the new tokens' dtype"
-    assert k.device == dev and v.device == dev, "caches must be on the new tokens' device"
-    ks = k.shape
-    assert len(ks) == 4 and v.shape == ks and ks[1] == Hkv and ks[3] == D, "caches must be [.., num_kv_heads, rows, head_dim], both alike"
+def check_caches(k: torch.Tensor, v: torch.Tensor, B: int, Hkv: int, D: int, dtype, dev: int, block_table: Optional[torch.Tensor]):
+    """What every entry asks of a dense or paged pair of caches.  Returns (k's pointer and strides, v's,
+    rows that a sequence can hold, table's pointer, its row stride, page_size, number of pages)."""
+    assert k.dtype is dtype and v.dtype is dtype, "cache dtype must equal the new tokens' dtype"
+    assert k.get_device() == dev and v.get_device() == dev, "caches must be on the new tokens' device"
+    shape = k.shape
+    assert len(shape) == 4 and v.shape == shape and shape[1] == Hkv and shape[3] == D, \
+        "caches must be [.., num_kv_heads, rows, head_dim], both alike"
+    kr, vr = rows_of(k), rows_of(v)
+    assert kr is not None and vr is not None, \
+        "caches must have 16-byte rows: unit stride in head_dim, other strides multiples of 8 elements, a 16-byte aligned base"
     if block_table is None:
-        assert ks[0] >= B, "dense caches must be [bsz, num_kv_heads, ctx, head_dim]"
-        return ks[2]
-    assert ks[2] % 64 == 0 and ks[2] > 0, "page_size must be a multiple of 64"
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.size(0) == B and block_table.device == dev \
-        and block_table.stride(1) == 1, "block_table must be [bsz, max_pages] int32 on the caches' device, unit stride along a row"
-    return block_table.size(1) * ks[2]
+        assert shape[0] >= B, "dense caches must be [bsz, num_kv_heads, ctx, head_dim]"
+        return kr, vr, shape[2], 0, 0, 0, 0
+    page = shape[2]
+    assert page % 64 == 0 and page > 0, "page_size must be a multiple of 64"
+    assert block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.get_device() == dev
+    rows, width = block_table.shape
+    stride, one = block_table.stride()
+    assert rows == B and (one == 1 or width <= 1), "block_table must be [bsz, max_pages] int32 on the caches' device, unit stride along a row"
+    return kr, vr, width * page, block_table.data_ptr(), stride, page, shape[0]
+
+
+def check_in_place(k: torch.Tensor, v: torch.Tensor, kv_seq_len: torch.Tensor, B: int) -> None:
+    assert not _overlaps(k) and not _overlaps(v), "caches are updated in place and must not be expanded"
+    assert B <= 1 or kv_seq_len.stride(0) == 1, "kv_seq_len is updated in place and must be contiguous"
+
+
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether some dimension is broadcast (stride 0)."""
+    return 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+
+
+def check_weights(w: torch.Tensor, B: int, Hkv: int, ctx: int, dev: int):
+    """(pointer, strides of the two leading dimensions)"""
+    b, h, n = w.shape
+    sb, sh, one = w.stride()
+    assert w.dtype is _f32 and w.get_device() == dev and b == B and h == Hkv and n >= ctx and (one == 1 or n <= 1) and not _overlaps(w), \
+        "row_weights must be [bsz, num_kv_heads, ctx] fp32 on the caches' device, unit stride along ctx"
+    return w.data_ptr(), sb, sh
 
 
 def _decode(q, k, v, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv_group_num, softcap, alibi_slopes, window, row_weights,
@@ -46,72 +80,64 @@ def _decode(q, k, v, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv
         raise RuntimeError("decode_attention runs on CUDA tensors only (no CPU path exists)")
     B, H, one, D = q.shape
     dt = q.dtype
-    dev = q.device
-    assert one == 1, "q must be [bsz, num_heads, 1, head_dim]: one new token per sequence"
-    assert D in (32, 64, 128, 256)
-    assert dt in _DT, "q must be fp16 or bf16"
+    dev = q.get_device()
+    code = _DT.get(dt)
     G = int(kv_group_num)
+    assert one == 1, "q must be [bsz, num_heads, 1, head_dim]: one new token per sequence"
+    assert D in _HEAD_DIMS and code is not None, "q must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
     assert G >= 1 and H % G == 0, "num_heads must be a multiple of kv_group_num"
     Hkv = H // G
-    ctx = _check_caches(k, v, B, Hkv, D, dt, dev, block_table)
-    _check_lengths(kv_seq_len, B, dev)
+    kr, vr, ctx, table, table_sb, page, n_pages = check_caches(k, v, B, Hkv, D, dt, dev, block_table)
+    is64 = check_lengths(kv_seq_len, B, dev)
     if max_seq_len_in_batch is not None:
         ctx = min(ctx, int(max_seq_len_in_batch))
-    if not rows_ok(q):
+    qr = rows_of(q)
+    if qr is None:
         q = q.clone(memory_format=torch.contiguous_format)
-    assert rows_ok(k) and rows_ok(v), "caches must have 16-byte rows: unit stride in head_dim, other strides multiples of 8 elements"
-    if not kv_seq_len.is_contiguous():
+        qr = rows_of(q)
+    if B > 1 and kv_seq_len.stride(0) != 1:
         kv_seq_len = kv_seq_len.contiguous()
-    cap = 0.0
     if softcap is not None:
-        cap = float(softcap)
-        assert cap > 0.0 and math.isfinite(cap), "softcap must be positive"
+        softcap = float(softcap)
+        assert 0.0 < softcap < math.inf, "softcap must be positive"
     if window is not None:
-        assert int(window) > 0, "window must be positive"
+        window = min(int(window), 0x7fffffff)
+        assert window > 0, "window must be positive"
     slopes = 0
     if alibi_slopes is not None:
-        assert alibi_slopes.dtype == torch.float32 and alibi_slopes.shape == (H,) and alibi_slopes.device == dev \
+        assert alibi_slopes.dtype is _f32 and alibi_slopes.shape == (H,) and alibi_slopes.get_device() == dev \
             and alibi_slopes.is_contiguous(), "alibi_slopes must be [num_heads] fp32 on q's device"
         slopes = alibi_slopes.data_ptr()
-    rw, rw_sb, rw_sh = 0, 0, 0
-    if row_weights is not None:
-        assert row_weights.dtype == torch.float32 and row_weights.dim() == 3 and row_weights.device == dev \
-            and row_weights.size(0) == B and row_weights.size(1) == Hkv and row_weights.size(2) >= ctx and row_weights.stride(2) == 1 \
-            and not _overlaps(row_weights), "row_weights must be [bsz, num_kv_heads, ctx] fp32 on q's device, unit stride along ctx"
-        rw, rw_sb, rw_sh = row_weights.data_ptr(), row_weights.stride(0), row_weights.stride(1)
-    out = torch.empty((B, H, 1, D), dtype=dt, device=dev)
-    lse = torch.empty((B, H, 1), dtype=torch.float32, device=dev) if return_lse else None
-    if B == 0:
-        return (out, lse) if return_lse else out
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    paged = block_table is not None
-    with on_device(dev) as stream:
-        size = _workspace(lib, dev.index, B, H, Hkv, D, ctx, dt, row_weights is not None, grid)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        p = _lib.pack_token(
-            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-            kv_seq_len.data_ptr(), block_table.data_ptr() if paged else 0, block_table.stride(0) if paged else 0, slopes,
-            out.data_ptr(), H * D, D, lse.data_ptr() if return_lse else 0, H, rw, rw_sb, rw_sh, ws.data_ptr(), size,
-            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), cap, 0 if window is None else min(int(window), 0x7fffffff),
-            1 if kv_seq_len.dtype == torch.int64 else 0, B, H, Hkv, D, ctx, k.size(2) if paged else 0, k.size(0) if paged else 0,
-            _DT[dt], grid, 0)
-        _lib.check(lib.fta_decode_token(p, stream), "fta_decode_token")
+    weights = row_weights is not None
+    rw, rw_sb, rw_sh = check_weights(row_weights, B, Hkv, ctx, dev) if weights else (0, 0, 0)
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, H, 1, D), dtype=dt, device=q.device)
+    lse = torch.empty((B, H, 1), dtype=_f32, device=q.device) if return_lse else None
+    if B and H:
+        size = _workspace(lib, dev, B, H, Hkv, D, ctx, code, weights, grid)
+        ws = out.new_empty(size)  # `size` elements of two bytes each
+        launch(lib.fta_decode_token, pack_token(
+            qr[0], qr[1], qr[2], *kr, *vr, kv_seq_len.data_ptr(), table, table_sb, slopes, out.data_ptr(), H * D, D,
+            lse.data_ptr() if return_lse else 0, H, rw, rw_sb, rw_sh, ws.data_ptr(), 2 * size,
+            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), softcap or 0.0, window or 0, is64,
+            B, H, Hkv, D, ctx, page, n_pages, code, grid, 0), dev, "fta_decode_token")
     return (out, lse) if return_lse else out
 
 
-_ws_sizes = {}  # sizes -> bytes of workspace: a function of the sizes and the device alone
+_ws_sizes = {}  # sizes -> 16-bit elements of workspace: a function of the sizes and the device alone
 
 
-def _workspace(lib, index, B, H, Hkv, D, ctx, dt, weights, grid) -> int:
-    key = (index, B, H, Hkv, D, ctx if weights else 0, dt, weights, grid)
+def _workspace(lib, *key) -> int:
     size = _ws_sizes.get(key)
     if size is None:
+        index, B, H, Hkv, D, ctx, code, weights, grid = key
         p = _lib.FtaTokenParams()
-        p.B, p.H, p.Hkv, p.D, p.ctx, p.dtype, p.grid_override = B, H, Hkv, D, ctx, _DT[dt], grid
+        p.B, p.H, p.Hkv, p.D, p.ctx, p.dtype, p.grid_override = B, H, Hkv, D, ctx, code, grid
         p.row_weights = 1 if weights else 0
-        size = lib.fta_decode_token_workspace_bytes(_lib.byref(p))
+        with torch.cuda.device(index):
+            size = lib.fta_decode_token_workspace_bytes(_lib.byref(p))
         if size < 0:
             raise _lib.FtaError(-size, "fta_decode_token_workspace_bytes")
+        size = (size + 1) // 2
         if len(_ws_sizes) >= 4096:
             _ws_sizes.clear()
         _ws_sizes[key] = size
@@ -183,36 +209,21 @@ def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: i
     lib = _lib.load()
     if not k_cache.is_cuda:
         raise RuntimeError("evict_rows runs on CUDA tensors only (no CPU path exists)")
-    dt, dev = k_cache.dtype, k_cache.device
-    assert dt in _DT and k_cache.dim() == 4, "caches must be fp16 or bf16 [.., num_kv_heads, rows, head_dim]"
-    B, Hkv, D = kv_seq_len.size(0) if kv_seq_len.dim() == 1 else -1, k_cache.size(1), k_cache.size(3)
-    assert D in (32, 64, 128, 256)
-    ctx = _check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
-    _check_lengths(kv_seq_len, B, dev)
-    assert rows_ok(k_cache) and rows_ok(v_cache) and not _overlaps(k_cache) and not _overlaps(v_cache), \
-        "caches are updated in place: they must have 16-byte rows and must not be expanded"
-    assert B <= 1 or kv_seq_len.stride(0) == 1, "kv_seq_len is updated in place and must be contiguous"
-    assert row_weights.dtype == torch.float32 and row_weights.dim() == 3 and row_weights.device == dev and row_weights.size(0) == B \
-        and row_weights.size(1) == Hkv and row_weights.size(2) >= ctx and row_weights.stride(2) == 1 and not _overlaps(row_weights), \
-        "row_weights must be [bsz, num_kv_heads, ctx] fp32 on the caches' device, unit stride along ctx"
+    dt, dev = k_cache.dtype, k_cache.get_device()
+    assert dt in _DT and k_cache.dim() == 4 and kv_seq_len.dim() == 1, \
+        "caches must be fp16 or bf16 [.., num_kv_heads, rows, head_dim], kv_seq_len [bsz]"
+    B = kv_seq_len.size(0)
+    _, Hkv, _, D = k_cache.shape
+    assert D in _HEAD_DIMS, "head_dim must be 32, 64, 128 or 256"
+    kr, vr, ctx, table, table_sb, page, n_pages = check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
+    is64 = check_lengths(kv_seq_len, B, dev)
+    check_in_place(k_cache, v_cache, kv_seq_len, B)
+    assert row_weights.dim() == 3, "row_weights must be [bsz, num_kv_heads, ctx]"
+    rw, rw_sb, rw_sh = check_weights(row_weights, B, Hkv, ctx, dev)
     budget, recent = int(budget), int(recent)
     assert 1 <= budget <= 0x7fffffff and 0 <= recent <= budget, "1 <= budget and 0 <= recent <= budget"
-    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
-    if B == 0:
-        return kept
-    ks, vs = k_cache.stride(), v_cache.stride()
-    paged = block_table is not None
-    p = _lib.pack_evict(
-        k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2], kv_seq_len.data_ptr(),
-        block_table.data_ptr() if paged else 0, block_table.stride(0) if paged else 0,
-        row_weights.data_ptr(), row_weights.stride(0), row_weights.stride(1), kept.data_ptr(),
-        1 if kv_seq_len.dtype == torch.int64 else 0, B, Hkv, D, ctx, k_cache.size(2) if paged else 0, k_cache.size(0) if paged else 0,
-        budget, recent, 0)
-    with on_device(dev) as stream:
-        _lib.check(lib.fta_evict_rows(p, stream), "fta_evict_rows")
+    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_cache.device)
+    if B and Hkv:
+        launch(lib.fta_evict_rows, pack_evict(*kr, *vr, kv_seq_len.data_ptr(), table, table_sb, rw, rw_sb, rw_sh, kept.data_ptr(),
+                                              is64, B, Hkv, D, ctx, page, n_pages, budget, recent, 0), dev, "fta_evict_rows")
     return kept
-
-
-def _overlaps(t: torch.Tensor) -> bool:
-    """Whether some dimension of an in-place argument is broadcast (stride 0)."""
-    return any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))

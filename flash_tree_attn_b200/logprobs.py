@@ -10,9 +10,10 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._lib import on_device
+from ._lib import launch, pack_logprob
 
 _DT = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_LEN = {torch.int32: 0, torch.int64: 1}  # -> is int64
 MAX_TOP_K = 64
 
 
@@ -41,41 +42,43 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     lib = _lib.load()
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs runs on CUDA tensors only (no CPU path exists)")
-    dev, dt = logits.device, logits.dtype
-    assert dt in _DT, "logits must be fp16, bf16 or fp32"
-    assert logits.dim() >= 1 and logits.size(-1) > 0, "logits must be [.., vocab]"
-    lead, V = logits.shape[:-1], logits.size(-1)
+    dev, code = logits.get_device(), _DT.get(logits.dtype)
+    shape = logits.shape
+    assert code is not None and len(shape) >= 1 and shape[-1] > 0, "logits must be [.., vocab] fp16, bf16 or fp32"
+    lead, V = shape[:-1], shape[-1]
     top_k = int(top_k)
-    assert 0 <= top_k <= min(MAX_TOP_K, V), "top_k must be 0 to 64 and at most the vocabulary"
-    if logits.dim() != 2:
+    assert 0 <= top_k <= MAX_TOP_K and top_k <= V, "top_k must be 0 to 64 and at most the vocabulary"
+    if len(shape) != 2:
         logits = logits.reshape(-1, V)
     rows = logits.size(0)
-    if V > 1 and logits.stride(1) != 1:
+    row_stride, one = logits.stride()
+    if one != 1 and V > 1:
         logits = logits.contiguous()
-    n, tp, tsr, t64, lp = 0, 0, 0, 0, None
+        row_stride = V
+    n = tp = token_stride = t64 = 0
+    lp = None
     if tokens is not None:
-        assert tokens.dtype in (torch.int32, torch.int64) and tokens.device == dev and tokens.dim() == len(lead) + 1 \
-            and tokens.shape[:-1] == lead, "tokens must be [.., n] int32 or int64 on the logits' device, with the logits' leading sizes"
-        n = tokens.size(-1)
-        if tokens.dim() != 2:
+        t64 = _LEN.get(tokens.dtype)
+        ts = tokens.shape
+        assert t64 is not None and tokens.get_device() == dev and len(ts) == len(shape) and ts[:-1] == lead, \
+            "tokens must be [.., n] int32 or int64 on the logits' device, with the logits' leading sizes"
+        n = ts[-1]
+        if len(ts) != 2:
             tokens = tokens.reshape(rows, n)
-        if n > 1 and tokens.stride(1) != 1:
+        token_stride, one = tokens.stride()
+        if one != 1 and n > 1:
             tokens = tokens.contiguous()
-        tp, tsr, t64 = tokens.data_ptr(), tokens.stride(0), 1 if tokens.dtype == torch.int64 else 0
-        lp = torch.empty((*lead, n), dtype=torch.float32, device=dev)
-    entropy, lse = torch.empty((2, *lead), dtype=torch.float32, device=dev).unbind(0)
+            token_stride = n
+        tp = tokens.data_ptr()
+        lp = torch.empty((*lead, n), dtype=torch.float32, device=logits.device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    lse = torch.empty_like(entropy)
     top_lp = top_ids = None
     if top_k:
-        top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=dev)
-        top_ids = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
+        top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=logits.device)
+        top_ids = torch.empty((*lead, top_k), dtype=torch.int64, device=logits.device)
     if rows:
-        with on_device(dev) as stream:
-            p = [logits.data_ptr(), logits.stride(0), tp, tsr, lp.data_ptr() if n else 0, entropy.data_ptr(), lse.data_ptr(),
-                 top_lp.data_ptr() if top_k else 0, top_ids.data_ptr() if top_k else 0, 0, 0, rows, V, n, top_k, _DT[dt], t64]
-            size = lib.fta_token_logprobs_workspace_bytes(_lib.pack_logprob(*p))
-            if size < 0:
-                raise _lib.FtaError(-size, "fta_token_logprobs_workspace_bytes")
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            p[9], p[10] = ws.data_ptr(), size
-            _lib.check(lib.fta_token_logprobs(_lib.pack_logprob(*p), stream), "fta_token_logprobs")
+        launch(lib.fta_token_logprobs, pack_logprob(
+            logits.data_ptr(), row_stride, tp, token_stride, lp.data_ptr() if n else 0, entropy.data_ptr(), lse.data_ptr(),
+            top_lp.data_ptr() if top_k else 0, top_ids.data_ptr() if top_k else 0, rows, V, n, top_k, code, t64), dev, "fta_token_logprobs")
     return TokenLogprobs(lp, entropy, lse, top_lp, top_ids)

@@ -13,8 +13,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import on_device, rows_ok
-from .decode import _DT, _LEN, _check_caches, _check_lengths, _overlaps
+from ._lib import launch, pack_rotary, rows_of
+from .decode import _DT, _HEAD_DIMS, _LEN, check_caches, check_in_place, check_lengths
 
 _LAYOUT = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
 
@@ -57,33 +57,36 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
     return torch.tensor([f * x + f / factor * (1.0 - x) for f, x in zip(plain, keep)], dtype=torch.float64, device=device), amplitude
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor):
+    """(the tensor or a copy of it with rows that can be copied in 16-byte pieces, its pointer and strides)"""
+    r = rows_of(t)
+    if r is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        r = rows_of(t)
+    return t, r
 
 
-def _check_frequencies(inv_freq: torch.Tensor, D: int, dev, layout: str) -> int:
-    assert layout in _LAYOUT, "layout: half or interleaved"
-    n = inv_freq.numel()
-    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.device == dev and inv_freq.is_contiguous(), \
+def _check_frequencies(inv_freq: torch.Tensor, D: int, dev: int, layout: str):
+    """(number of pairs, layout's code)"""
+    code = _LAYOUT.get(layout)
+    assert code is not None, "layout: half or interleaved"
+    assert inv_freq.dtype is torch.float64 and inv_freq.dim() == 1 and inv_freq.get_device() == dev and inv_freq.is_contiguous(), \
         "inv_freq must be a contiguous float64 vector on q's device"
+    n = inv_freq.size(0)
     assert n > 0 and n % 8 == 0 and 2 * n <= D, "inv_freq must have a multiple of 8 entries, at most head_dim / 2"
-    return n
+    return n, code
 
 
-def _check_positions(positions: torch.Tensor, offsets: Optional[torch.Tensor], B: int, Q: int, dev):
-    """-> (pointer, stride along bsz, stride along q_len, is int64, offsets' pointer)"""
-    assert positions.dtype in _LEN and positions.device == dev and tuple(positions.shape) in ((B,), (B, Q)), \
+def _check_positions(positions: torch.Tensor, B: int, Q: int, dev: int):
+    """(the tensor or a copy, its pointer, stride along bsz, stride along q_len (0: consecutive positions), is int64)"""
+    is64, shape = _LEN.get(positions.dtype), positions.shape
+    assert is64 is not None and positions.get_device() == dev and (shape == (B,) or shape == (B, Q)), \
         "positions must be [bsz] or [bsz, q_len] int32 or int64 on q's device"
-    if offsets is not None:
-        assert offsets.dtype == torch.int32 and offsets.shape == (Q,) and offsets.device == dev and offsets.is_contiguous(), \
-            "offsets must be [q_len] int32 on q's device"
-    each = positions.dim() == 2
-    if each and positions.stride(1) == 0:  # the same position for every token: stride 0 would mean consecutive ones
-        positions = positions.contiguous()
-        if positions.stride(1) == 0:
-            positions = positions.clone(memory_format=torch.contiguous_format)
-    return positions, positions.stride(0), positions.stride(1) if each else 0, 1 if positions.dtype == torch.int64 else 0, \
-        0 if offsets is None else offsets.data_ptr()
+    if len(shape) == 1:
+        return positions, positions.data_ptr(), positions.stride(0), 0, is64
+    if positions.stride(1) == 0:  # the same position for every token: as a stride, 0 would mean consecutive ones
+        positions = positions.clone(memory_format=torch.contiguous_format)
+    return positions, positions.data_ptr(), positions.stride(0), positions.stride(1), is64
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -109,28 +112,30 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if not q.is_cuda:
         raise RuntimeError("apply_rotary runs on CUDA tensors only (no CPU path exists)")
     B, H, Q, D = q.shape
-    dt, dev = q.dtype, q.device
-    assert dt in _DT and D in (32, 64, 128, 256), "q must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
-    n = _check_frequencies(inv_freq, D, dev, layout)
-    q = _rows(q)
-    qo = torch.empty((B, H, Q, D), dtype=dt, device=dev)
-    Hkv, kp, ks, ko = 0, 0, (0, 0, 0), None
+    dt, dev = q.dtype, q.get_device()
+    code = _DT.get(dt)
+    assert code is not None and D in _HEAD_DIMS, "q must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
+    n, layout = _check_frequencies(inv_freq, D, dev, layout)
+    q, qr = _rows(q)
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    Hkv, kr, ko, kp = 0, (0, 0, 0, 0), None, 0
     if k is not None:
-        assert k.dtype == dt and k.device == dev and k.dim() == 4 and k.size(0) == B and k.size(2) == Q and k.size(3) == D, \
-            "k must be [bsz, num_kv_heads, q_len, head_dim] of q's dtype and on its device"
-        k = _rows(k)
-        Hkv, kp, ks = k.size(1), k.data_ptr(), k.stride()
-        ko = torch.empty((B, Hkv, Q, D), dtype=dt, device=dev)
-    positions, psb, psq, is64, off = _check_positions(positions, offsets, B, Q, dev)
-    if B == 0 or Q == 0 or H + Hkv == 0:
-        return qo, ko
-    qs = q.stride()
-    p = _lib.pack_rotary(
-        q.data_ptr(), qs[0], qs[1], qs[2], kp, ks[0], ks[1], ks[2], 0, 0, 0, 0, qo.data_ptr(), 0 if ko is None else ko.data_ptr(),
-        0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, positions.data_ptr(), psb, psq, off, inv_freq.data_ptr(),
-        float(amplitude), _LAYOUT[layout], 1 if inverse else 0, n, 0, is64, B, H, Hkv, Q, D, 0, 0, 0, _DT[dt], 0)
-    with on_device(dev) as stream:
-        _lib.check(lib.fta_apply_rotary(p, stream), "fta_apply_rotary")
+        assert k.dtype is dt and k.get_device() == dev and k.dim() == 4, "k must be of q's dtype and on its device"
+        kb, Hkv, kq, kd = k.shape
+        assert kb == B and kq == Q and kd == D, "k must be [bsz, num_kv_heads, q_len, head_dim]"
+        k, kr = _rows(k)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        kp = ko.data_ptr()
+    positions, pos, psb, psq, is64 = _check_positions(positions, B, Q, dev)
+    off = 0
+    if offsets is not None:
+        assert offsets.dtype is torch.int32 and offsets.shape == (Q,) and offsets.get_device() == dev and offsets.is_contiguous(), \
+            "offsets must be [q_len] int32 on q's device"
+        off = offsets.data_ptr()
+    if B and Q and H + Hkv:
+        launch(lib.fta_apply_rotary, pack_rotary(
+            *qr, *kr, 0, 0, 0, 0, qo.data_ptr(), kp, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, pos, psb, psq, off, inv_freq.data_ptr(),
+            float(amplitude), layout, 1 if inverse else 0, n, 0, is64, B, H, Hkv, Q, D, 0, 0, 0, code, 0), dev, "fta_apply_rotary")
     return qo, ko
 
 
@@ -155,38 +160,30 @@ def append_tokens(k_cache, v_cache, q, k, v, kv_seq_len, *, inv_freq: Optional[t
     if not k_cache.is_cuda:
         raise RuntimeError("append_tokens runs on CUDA tensors only (no CPU path exists)")
     B, Hkv, Q, D = k.shape
-    dt, dev = k.dtype, k_cache.device
-    assert dt in _DT and D in (32, 64, 128, 256), "k must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
-    assert k.device == dev and v.device == dev and v.dtype == dt and v.shape == k.shape, "k and v must be alike, on the caches' device"
-    ctx = _check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
-    _check_lengths(kv_seq_len, B, dev)
-    assert rows_ok(k_cache) and rows_ok(v_cache) and not _overlaps(k_cache) and not _overlaps(v_cache), \
-        "caches are updated in place: they must have 16-byte rows and must not be expanded"
-    assert B <= 1 or kv_seq_len.stride(0) == 1, "kv_seq_len is updated in place and must be contiguous"
-    assert q.dim() == 4 and q.size(0) == B and q.size(2) == Q and q.size(3) == D and q.dtype == dt and q.device == dev, \
+    dt, dev = k.dtype, k_cache.get_device()
+    code = _DT.get(dt)
+    assert code is not None and D in _HEAD_DIMS, "k must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
+    assert k.get_device() == dev and v.get_device() == dev and v.dtype is dt and v.shape == k.shape, "k and v must be alike, on the caches' device"
+    kc, vc, ctx, table, table_sb, page, n_pages = check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
+    len64 = check_lengths(kv_seq_len, B, dev)
+    check_in_place(k_cache, v_cache, kv_seq_len, B)
+    qb, H, qq, qd = q.shape
+    assert qb == B and qq == Q and qd == D and q.dtype is dt and q.get_device() == dev, \
         "q must be [bsz, num_heads, q_len, head_dim] of k's dtype and on its device"
-    n, out, H, qp, qs = 0, q, 0, 0, (0, 0, 0)
-    k, v = _rows(k), _rows(v)
-    psb = psq = is64 = pos = freq = 0
+    k, kr = _rows(k)
+    v, vr = _rows(v)
+    out, qr, qo, n, pos, psb, psq, is64, freq = q, (0, 0, 0, 0), 0, 0, 0, 0, 0, 0, 0
     if inv_freq is not None:
-        n = _check_frequencies(inv_freq, D, dev, layout)
-        H = q.size(1)
-        q = _rows(q)
-        out = torch.empty((B, H, Q, D), dtype=dt, device=dev)
-        qp, qs, freq = q.data_ptr(), q.stride(), inv_freq.data_ptr()
+        n, layout = _check_frequencies(inv_freq, D, dev, layout)
+        q, qr = _rows(q)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        qo, freq = out.data_ptr(), inv_freq.data_ptr()
         if positions is not None:
-            positions, psb, psq, is64, _ = _check_positions(positions, None, B, Q, dev)
-            pos = positions.data_ptr()
-    if B == 0 or Q == 0 or Hkv == 0:
-        return out
-    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
-    paged = block_table is not None
-    p = _lib.pack_rotary(
-        qp, qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr() if n else 0, 0,
-        k_cache.data_ptr(), kc[0], kc[1], kc[2], v_cache.data_ptr(), vc[0], vc[1], vc[2], kv_seq_len.data_ptr(),
-        block_table.data_ptr() if paged else 0, block_table.stride(0) if paged else 0, pos, psb, psq, 0, freq,
-        float(amplitude), _LAYOUT[layout], 0, n, 1 if kv_seq_len.dtype == torch.int64 else 0, is64, B, H, Hkv, Q, D, ctx,
-        k_cache.size(2) if paged else 0, k_cache.size(0) if paged else 0, _DT[dt], 0)
-    with on_device(dev) as stream:
-        _lib.check(lib.fta_append_tokens(p, stream), "fta_append_tokens")
+            positions, pos, psb, psq, is64 = _check_positions(positions, B, Q, dev)
+    else:
+        layout, H = 0, 0
+    if B and Q and Hkv:
+        launch(lib.fta_append_tokens, pack_rotary(
+            *qr, *kr, *vr, qo, 0, *kc, *vc, kv_seq_len.data_ptr(), table, table_sb, pos, psb, psq, 0, freq,
+            float(amplitude), layout, 0, n, len64, is64, B, H, Hkv, Q, D, ctx, page, n_pages, code, 0), dev, "fta_append_tokens")
     return out

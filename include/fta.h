@@ -390,15 +390,11 @@ typedef struct FtaLogprobParams {
   float* lse;          /* [rows] */
   float* top_logprobs; /* [rows, top_k] contiguous */
   int64_t* top_ids;    /* [rows, top_k] contiguous */
-  void* workspace;
-  int64_t workspace_bytes;
   int32_t rows, vocab, n_tokens, top_k;
   int32_t dtype; /* FTA_DTYPE_* */
   int32_t tokens_are_i64;
 } FtaLogprobParams;
 
-/* Bytes of workspace the call needs; negative: -FTA_E_*.  rows, vocab, top_k and dtype are read. */
-int64_t fta_token_logprobs_workspace_bytes(const FtaLogprobParams* p);
 int fta_token_logprobs(const FtaLogprobParams* p, void* stream);
 
 /* Text for an FTA_E_* code.  No counterpart in the reference (it raises AssertionError,

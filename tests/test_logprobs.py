@@ -42,7 +42,7 @@ def _tokens(rows, V, n, g, dtype=torch.int64):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,V,k", [(1, 1, 1), (3, 2, 2), (2, 7, 3), (5, 64, 64), (3, 100, 64), (2, 255, 5), (2, 2049, 20), (3, 4097, 64), (2, 16384, 1),
-                                      (2, 32768, 33), (2, 32769, 64), (300, 1000, 8), (3, 50257, 20), (2, 128256, 5), (1, 262144, 64), (4, 5000, 0)])
+                                      (2, 32768, 33), (2, 32769, 64), (300, 1000, 8), (3, 50257, 20), (2, 128256, 5), (1, 262144, 64), (2, 300001, 10), (4, 5000, 0)])
 def test_matches_the_formula(dtype, rows, V, k):
     import flash_tree_attn_b200 as fta
 
@@ -145,9 +145,9 @@ def test_leading_sizes_strides_capture_and_repeat():
 
 def _fake(**kw):
     p = _lib.FtaLogprobParams()
-    for name in ("logits", "tokens", "logprobs", "entropy", "lse", "top_logprobs", "top_ids", "workspace"):
+    for name in ("logits", "tokens", "logprobs", "entropy", "lse", "top_logprobs", "top_ids"):
         setattr(p, name, 4096)
-    p.l_sr, p.t_sr, p.rows, p.vocab, p.n_tokens, p.top_k, p.dtype, p.workspace_bytes = 100, 2, 3, 100, 2, 5, _lib.DTYPE_F16, 1 << 20
+    p.l_sr, p.t_sr, p.rows, p.vocab, p.n_tokens, p.top_k, p.dtype = 100, 2, 3, 100, 2, 5, _lib.DTYPE_F16
     for name, value in kw.items():
         setattr(p, name, value)
     return p
@@ -156,16 +156,14 @@ def _fake(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(rows=0), 1), (dict(vocab=0), 1), (dict(top_k=-1), 1), (dict(top_k=101), 1), (dict(n_tokens=-1), 1), (dict(dtype=3), 1), (dict(logits=None), 1),
     (dict(logits=4097), 1), (dict(entropy=None), 1), (dict(lse=None), 1), (dict(tokens=None), 1), (dict(logprobs=None), 1), (dict(top_ids=None), 1),
-    (dict(vocab=1 << 22, top_k=65), 2), (dict(vocab=(1 << 21) + 1), 2), (dict(workspace=None), 3), (dict(workspace=4100), 3), (dict(workspace_bytes=167), 3)])
+    (dict(top_k=65), 2), (dict(vocab=(1 << 21) + 1), 2), (dict(rows=(1 << 27) + 1), 2)])
 def test_c_entry_refuses(fta_lib, kw, code):
     assert fta_lib.fta_token_logprobs(C.byref(_fake(**kw)), None) == code
 
 
-def test_c_struct_and_sizes(fta_lib):
-    assert C.sizeof(_lib.FtaLogprobParams) == 112  # as a C++ compile of include/fta.h prints
+def test_c_struct_and_null(fta_lib):
+    assert C.sizeof(_lib.FtaLogprobParams) == 96  # as a C++ compile of include/fta.h prints
     assert fta_lib.fta_token_logprobs(None, None) == _lib.FTA_E_BADARG
-    assert fta_lib.fta_token_logprobs_workspace_bytes(C.byref(_fake())) == 3 * (16 + 8 * 5)
-    assert fta_lib.fta_token_logprobs_workspace_bytes(C.byref(_fake(dtype=7))) == -_lib.FTA_E_BADARG
 
 
 @pytest.mark.gpu
