@@ -5,25 +5,24 @@
 //   lse = m + log s,  entropy = log s - t / s,  log p(token) = x[token] - lse.
 // Every term of t has the same sign, so the entropy loses nothing but in the last difference.
 //
-// Where |m| < 30000 the exponents are x log2(e) - m2 with m2 = m log2(e) rounded, one fused multiply-add
-// an element; what the rounding of m2 shifts, r = m log2(e) - m2, is known exactly and taken out of the
-// piece's sums.  Elsewhere (logits masked with the type's lowest value and nothing else) they are
-// (x - m) log2(e), which cannot overflow.
-//
 // What bounds it: the logits are read once; with 16-bit logits an SM gets about 12 elements a clock from
-// memory, so there is room for about 10 instructions an element, and 16 exponentials a clock.  A row is
-// cut into pieces that a block holds in registers (8 chunks of 16 bytes a thread), so the maximum (packed,
-// per chunk), the sums (6 instructions an element) and the search for the likeliest need no second
-// read.  A row's pieces are a cluster's blocks (a block takes several of a row with more than 8): they
-// spread a few long rows over the machine, and join through distributed shared memory, without a
-// workspace or a second kernel.
+// memory, so there is room for about 10 instructions an element, and 16 exponentials a clock.  So each
+// thread keeps sums of its own against a reference of its own, which moves only when a logit passes it
+// by 14 (in 32 bits a ratio of sums does not care), with 6 instructions an element: the exponent is
+// x log2(e) - c, c = m log2(e) rounded, one fused multiply-add, and what the rounding of c shifts,
+// r = m log2(e) - c, is known exactly and taken out at the end.  Where |m| >= 30000 (logits masked with the
+// type's lowest value and nothing else) it is (x - m) log2(e), which cannot overflow.
 //
-// The likeliest of a piece: every warp's q-th largest of its lanes' maxima is a bound that at least q
-// of the warp's elements reach; the w-th largest of those bounds is reached by q w >= k elements.
-// Chunks whose maximum reaches it (typically less than twice k) are listed, their elements shared
-// out over the block, and those that reach it ranked by counting.  Looking at a chunk where it was found
-// would hold up its whole warp: a listed chunk costs a few instructions there.  Where too many reach the
-// bound (ties, masked vocabularies) the exact one is found bit by bit instead.
+// A row is walked in rounds of 8 chunks of 16 bytes a thread, by one block or, where there are few rows,
+// by the blocks of a cluster, which join through distributed shared memory: no workspace and no
+// second kernel.
+//
+// The likeliest: in the first round every warp's q-th largest lane maximum is a bound that at least q of
+// the warp's elements reach; the w-th largest of those bounds is reached by q w >= k elements.  Chunks
+// whose maximum reaches it (typically less than twice k; later, the k-th largest so far is the bound)
+// are listed, their elements shared out over the block and ranked by counting.  Looking at a chunk where
+// it was found would hold up its whole warp.  Where too many reach the bound (ties, masked vocabularies)
+// the exact one is found bit by bit instead.
 #include <cooperative_groups.h>
 
 #include "fta_common.cuh"
@@ -35,9 +34,10 @@ namespace {
 constexpr int kThreads = 256;     // 4 blocks an SM: one computes while the others' chunks arrive
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunks = 8;        // 16-byte chunks per thread
-constexpr int kListed = 1024;     // elements ranked by counting
-constexpr int kListedChunks = 256;
-constexpr int kMostRounds = 16;   // largest q; below 4 full warps a piece has fewer than kListed elements
+constexpr int kListedChunks = 128;
+constexpr int kListed = 8 * kListedChunks;  // elements ranked by counting
+constexpr int kPending = 64;      // listed chunks that may wait for the next round
+constexpr int kMostRounds = 16;   // largest q; below 4 full warps a row has fewer than kListedChunks
 constexpr int kMostBlocks = 8;    // of a cluster, so of a row
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -53,12 +53,11 @@ __device__ __forceinline__ void add_exp(float d, float& s, float& t) {
 }
 
 // A 16-byte chunk of logits.  max: NaN if any is.  add: sums over its elements for |m| < 30000; -inf is
-// raised to a value whose exponential is still 0, because 0 * -inf is NaN.  get: element i.
+// raised to a value whose exponential is still 0, because 0 * -inf is NaN.
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int n = 4;
   static constexpr uint32_t kLowest = 0xff800000u;  // -inf
-  static __device__ __forceinline__ uint32_t bits(const float* x) { return __float_as_uint(*x); }
   static __device__ __forceinline__ float max(const uint4& x) {
     return max_nan(max_nan(__uint_as_float(x.x), __uint_as_float(x.y)), max_nan(__uint_as_float(x.z), __uint_as_float(x.w)));
   }
@@ -67,12 +66,10 @@ template <> struct Vec<float> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) add_exp(max_nan(fmaf(__uint_as_float(w[i]), FTA_LOG2E, -m2), -1e30f), s, t);
   }
-  static __device__ __forceinline__ float get(uint32_t w, int) { return __uint_as_float(w); }
 };
 template <> struct Vec<__half> {
   static constexpr int n = 8;
   static constexpr uint32_t kLowest = 0xfc00u;
-  static __device__ __forceinline__ uint32_t bits(const __half* x) { return __half_as_ushort(*x); }
   static __device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
   static __device__ __forceinline__ float max(const uint4& x) {
     const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h2(x.x), h2(x.y)), __hmax2_nan(h2(x.z), h2(x.w))));
@@ -87,12 +84,10 @@ template <> struct Vec<__half> {
       add_exp(fmaf(f.y, FTA_LOG2E, -m2), s, t);
     }
   }
-  static __device__ __forceinline__ float get(uint32_t w, int i) { return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w & 0xffffu))); }
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int n = 8;
   static constexpr uint32_t kLowest = 0xff80u;
-  static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16* x) { return __bfloat16_as_ushort(*x); }
   static __device__ __forceinline__ __nv_bfloat162 b2(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
   static __device__ __forceinline__ uint32_t word(__nv_bfloat162 x) { return *reinterpret_cast<const uint32_t*>(&x); }
   static __device__ __forceinline__ float max(const uint4& x) {
@@ -108,7 +103,6 @@ template <> struct Vec<__nv_bfloat16> {
       add_exp(fmaf(__uint_as_float(y & 0xffff0000u), FTA_LOG2E, -m2), s, t);
     }
   }
-  static __device__ __forceinline__ float get(uint32_t w, int i) { return __uint_as_float(i ? w & 0xffff0000u : w << 16); }
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -131,7 +125,7 @@ __device__ __forceinline__ unsigned long long rank_key(uint32_t k, int token) {
   return ((unsigned long long)k << 32) | (uint32_t)(0xffffffffu - (uint32_t)token);
 }
 
-struct Sums { float m, s, t; };  // s and t in log2 units relative to m
+struct Sums { float m, s, t; };  // s and t (log2 units) relative to m
 
 template <int N> __device__ __forceinline__ int block_sum(int x, int* scratch) {
   x = __reduce_add_sync(0xffffffffu, x);
@@ -166,30 +160,32 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   return Sums{m, fa * a.s + fb * b.s, (fa == 0.f ? 0.f : fa * (a.t + da * a.s)) + (fb == 0.f ? 0.f : fb * (b.t + db * b.s))};
 }
 
-// grid = rows * (blocks of a cluster); block i of a row takes its pieces [i * rounds, (i + 1) * rounds).
-// Chunks lie on 16-byte boundaries of memory, whatever the row's start: element e of the row is element
-// e + head of the chunks.
+// grid = rows * (blocks of a cluster); block i of a row takes its rounds [i * rounds, (i + 1) * rounds) of
+// kThreads * kChunks chunks.  Chunks lie on 16-byte boundaries of memory, whatever the row's start; the few
+// elements before the first and behind the last are handed to one lane each.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobParams p, const int blocks, const int rounds) {
   constexpr int VE = Vec<T>::n;
-  static_assert(kThreads * kChunks * VE <= 1 << 15, "the search over a piece's tokens takes 16 steps");
-  __shared__ __align__(16) unsigned long long list[kListed + FTA_MAX_TOP_K + 8];
+  constexpr int kRound = kThreads * kChunks;
+  static_assert(kRound * VE <= 1 << 15, "the search over a round's tokens takes 16 steps");
+  __shared__ __align__(16) unsigned long long list[kListed + 2 * VE + FTA_MAX_TOP_K + 8];
   __shared__ unsigned long long best[FTA_MAX_TOP_K];  // the likeliest so far, in order; 0: none
   __shared__ Sums s_sums;
   __shared__ float s_a[kWarps], s_b[kWarps], s_c[kWarps];
   __shared__ int s_i[kWarps];
   __shared__ uint32_t s_key[kWarps];
   __shared__ int s_n, s_listed;
-  __shared__ uint4 s_chunk[kListedChunks];
   __shared__ int s_where[kListedChunks];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long row = blockIdx.x / blocks;
   const int block = blockIdx.x - (int)row * blocks;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.l_sr;
   const int head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int start = min(head ? VE - head : 0, p.vocab);  // the first chunk's first element
+  const int total = (p.vocab - start) / VE;               // chunks
   const int k = p.top_k;
-  Sums sums = {-INFINITY, 0.f, 0.f};
   if (tid < k) best[tid] = 0;
+  if (tid == 0) s_n = s_listed = 0;
   // the first block of a row answers for its tokens; their logits are asked for before all else
   auto logit_of = [&](int i, bool& inside) {
     const long long tok = p.tokens_are_i64 ? reinterpret_cast<const long long*>(p.tokens)[row * p.t_sr + i]
@@ -200,129 +196,135 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
   bool asked_inside = false;
   const float asked = block == 0 && tid < p.n_tokens ? logit_of(tid, asked_inside) : 0.f;
 
+  // the thread's reference, its rounded log2(e) multiple, what that rounding shifts, and the sums
+  float m = -INFINITY, c2 = 0.f, r = 0.f, s = 0.f, t = 0.f, limit = -INFINITY;
+  bool near = true;
+  float bound = -INFINITY;
+  int pending = 0;  // listed chunks that wait
   for (int round = 0; round < rounds; ++round) {
-    const int base = (block * rounds + round) * (kThreads * kChunks);  // first chunk of the piece
-    const int chunks = min(kThreads * kChunks, fta_cdiv(p.vocab + head, VE) - base);
-    if (chunks <= 0) break;
-    __syncthreads();  // the round before is done with the shared arrays
+    const int base = (block * rounds + round) * kRound;  // first chunk of the round
+    const int chunks = min(kRound, total - base);
+    if (round > 0) {
+      if (chunks <= 0) break;
+      if (k > 0) __syncthreads();  // everybody has read the round before's count
+    }
+    const uint4* at = reinterpret_cast<const uint4*>(x + start + (long long)(base + tid) * VE);
     uint4 raw[kChunks];
+    if (chunks == kRound) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int e0 = (base + c * kThreads + tid) * VE - head;
-      if (e0 >= 0 && e0 + VE <= p.vocab) {
-        raw[c] = __ldcs(reinterpret_cast<const uint4*>(x + e0));
-      } else {  // the row's ends
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
+      for (int c = 0; c < kChunks; ++c) raw[c] = __ldcs(at + c * kThreads);
+    } else {
+      const uint32_t low = VE == 8 ? Vec<T>::kLowest * 0x10001u : Vec<T>::kLowest;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const uint32_t v = e0 + i >= 0 && e0 + i < p.vocab ? Vec<T>::bits(x + e0 + i) : Vec<T>::kLowest;
-          w[i * 4 / VE] |= v << (VE == 8 ? 16 * (i & 1) : 0);
-        }
-        raw[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int c = 0; c < kChunks; ++c) {
+        raw[c] = make_uint4(low, low, low, low);
+        if (c * kThreads + tid < chunks) raw[c] = __ldcs(at + c * kThreads);
       }
     }
-    float top[kChunks], mine = -INFINITY;
+    // lane i of the row's first warp has the i-th element outside the chunks
+    int edge = -1;
+    float edge_logit = -INFINITY;
+    if (block == 0 && round == 0) {
+      edge = tid < start ? tid : total * VE + tid;
+      if (edge >= p.vocab) edge = -1;
+      if (edge >= 0) edge_logit = to_float(x[edge]);
+    }
+
+    float top[kChunks], mine = edge_logit;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       top[c] = Vec<T>::max(raw[c]);
-      mine = fmaxf(mine, top[c]);
+      mine = max_nan(mine, top[c]);
     }
-    float m = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (mine != mine) {  // so are the row's sums, whatever else the thread has
+      s = NAN;
+      mine = -INFINITY;
+    }
 
-    // the warp's bound: its q-th largest lane maximum
-    const int full = min(kWarps, chunks / 32);   // warps whose lanes all hold elements
-    const int q = full > 0 ? fta_cdiv(k, full) : kMostRounds + 1;
-    const bool bounded = k > 0 && q <= kMostRounds;
-    uint32_t kth = 0;
-    if (bounded && warp < full) {
-      uint32_t key = ordered(mine);
-      for (int i = 0; i < q; ++i) {
-        kth = __reduce_max_sync(0xffffffffu, key);
-        const unsigned who = __ballot_sync(0xffffffffu, key == kth);
-        if (lane == __ffs(who) - 1) key = 0;
+    if (round == 0 && k > 0) {
+      const int full = min(kWarps, chunks / 32);  // warps whose lanes all hold elements
+      const int q = full > 0 ? fta_cdiv(k, full) : kMostRounds + 1;
+      uint32_t kth = 0;
+      if (q <= kMostRounds && warp < full) {  // the warp's q-th largest lane maximum
+        uint32_t key = ordered(mine);
+        for (int i = 0; i < q; ++i) {
+          kth = __reduce_max_sync(0xffffffffu, key);
+          const unsigned who = __ballot_sync(0xffffffffu, key == kth);
+          if (lane == __ffs(who) - 1) key = 0;
+        }
+      }
+      if (lane == 0) s_key[warp] = kth;
+      __syncthreads();
+      if (q <= kMostRounds) {  // the w-th largest of those: the one that w - 1 others come before
+        kth = s_key[lane % kWarps];
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          const uint32_t o = __shfl_sync(0xffffffffu, kth, i);
+          before += o > kth || (o == kth && i < lane % kWarps);
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, before == fta_cdiv(k, q) - 1);
+        bound = unordered(__shfl_sync(0xffffffffu, kth, __ffs(who) - 1));
       }
     }
-    if (lane == 0) { s_a[warp] = m; s_key[warp] = kth; }
-    if (tid == 0) s_n = s_listed = 0;
-    __syncthreads();
-    m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_a[w]);
-    float bound = -INFINITY;
-    if (bounded) {  // the w-th largest of the warps' bounds: the one that w - 1 others come before
-      kth = s_key[lane % kWarps];
-      int before = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const uint32_t o = __shfl_sync(0xffffffffu, kth, i);
-        before += o > kth || (o == kth && i < lane % kWarps);
-      }
-      const unsigned who = __ballot_sync(0xffffffffu, before == fta_cdiv(k, q) - 1);
-      bound = unordered(__shfl_sync(0xffffffffu, kth, __ffs(who) - 1));
-    }
-    // what came in earlier rounds need not be reached again; a NaN there stays out of the comparison
-    if (k > 0 && best[k - 1] != 0) bound = fmaxf(bound, unordered((uint32_t)(best[k - 1] >> 32)));
 
-    const bool near = fabsf(m) < 30000.f;
-    const float m2 = __fmul_rn(m, FTA_LOG2E), safe = m == -INFINITY ? 0.f : m;
-    float s = 0.f, t = 0.f;
-    if (near) {
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        if (c * kThreads < chunks) Vec<T>::add(raw[c], m2, s, t);
-    } else {
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-        for (int i = 0; i < VE; ++i) add_exp(max_nan((Vec<T>::get(w[i * 4 / VE], i & 1) - safe) * FTA_LOG2E, -1e30f), s, t);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      t += __shfl_xor_sync(0xffffffffu, t, o);
-    }
-    __syncthreads();
-    if (lane == 0) { s_b[warp] = s; s_c[warp] = t; }
-    __syncthreads();
-    s = t = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) { s += s_b[w]; t += s_c[w]; }
-    if (near) {  // 2^(x log2(e) - m2) = e^(x - m) 2^r
-      const float r = fmaf(m, FTA_LOG2E, -m2), f = fta_exp2(-r);
-      t = f * (t - r * s);
+    if (mine > limit) {
+      const float to2 = __fmul_rn(mine, FTA_LOG2E);
+      near = fabsf(mine) < 30000.f;
+      const float r_to = near ? fmaf(mine, FTA_LOG2E, -to2) : 0.f;
+      const float shift = (m - mine) * FTA_LOG2E - r + r_to, f = fta_exp2(shift);
+      t = f == 0.f ? 0.f : f * (t + shift * s);
       s *= f;
+      m = mine; c2 = to2; r = r_to;
+      limit = mine + 14.f;
     }
-    sums = join(sums, Sums{m, s, t});
+    if (mine != -INFINITY) {
+      if (near) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          if (c * kThreads >= chunks) break;
+          float s1 = 0.f, t1 = 0.f;  // summed per chunk first: the sums' paths stay short
+          Vec<T>::add(raw[c], c2, s1, t1);
+          s += s1;
+          t += t1;
+        }
+        if (edge >= 0) add_exp(max_nan(fmaf(edge_logit, FTA_LOG2E, -c2), -1e30f), s, t);
+      } else {
+        for (int c = tid; c < chunks; c += kThreads)
+          for (int i = 0; i < VE; ++i) add_exp(max_nan((to_float(x[start + (base + c) * VE + i]) - m) * FTA_LOG2E, -1e30f), s, t);
+        if (edge >= 0) add_exp(max_nan((edge_logit - m) * FTA_LOG2E, -1e30f), s, t);
+      }
+    }
     if (k == 0) continue;
 
-    // list the chunks that reach the bound (NaN does), then their elements
+    // list the chunks that reach the bound (NaN does)
+    uint32_t reach = 0;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      if (top[c] < bound || c * kThreads + tid >= chunks) continue;
-      const int at = atomicAdd(&s_n, 1);
-      if (at < kListedChunks) {
-        s_chunk[at] = raw[c];
-        s_where[at] = c * kThreads + tid;
-      }
+    for (int c = 0; c < kChunks; ++c) reach |= top[c] < bound ? 0u : 1u << c;
+    while (reach != 0) {
+      const int c = (__ffs(reach) - 1) * kThreads + tid;
+      reach &= reach - 1;
+      if (c >= chunks) break;
+      const int to = atomicAdd(&s_n, 1);
+      if (to < kListedChunks) s_where[to] = base + c;
     }
+    if (edge >= 0 && !(edge_logit < bound)) list[atomicAdd(&s_listed, 1)] = rank_key(ordered(edge_logit), edge);
     __syncthreads();
     const int reached = s_n;
-    for (int i = tid; i < min(reached, kListedChunks) * VE; i += kThreads) {
-      const int at = i / VE, e = i % VE;
-      const float v = Vec<T>::get(reinterpret_cast<const uint32_t*>(&s_chunk[at])[e * 4 / VE], e & 1);
-      const int tok = (base + s_where[at]) * VE - head + e;
-      if (v < bound || tok < 0 || tok >= p.vocab) continue;
-      const int to = atomicAdd(&s_listed, 1);
-      if (to < kListed) list[to] = rank_key(ordered(v), tok);
+    if (round > 0 && round + 1 < rounds && base + kRound < total && reached <= kPending) {
+      pending = reached;
+      continue;
+    }
+    const bool over = reached > kListedChunks;
+    const int listed = over ? pending : reached;  // what earlier rounds listed comes first
+    for (int i = tid; i < listed * VE; i += kThreads) {
+      const int tok = start + s_where[i / VE] * VE + i % VE;
+      const float v = to_float(x[tok]);
+      if (!(v < bound)) list[atomicAdd(&s_listed, 1)] = rank_key(ordered(v), tok);
     }
     __syncthreads();
-    int n = s_listed;
-    if (reached > kListedChunks || n > kListed) {
-      const int lo = max(0, base * VE - head), hi = min(p.vocab, (base + kThreads * kChunks) * VE - head);
+    if (over) {
+      const int lo = start + base * VE, hi = lo + chunks * VE;
       // The k-th largest value, bit by bit from the top: the largest key that at least k elements reach.
       uint32_t key = 0;
       for (int bit = 31; bit >= 0; --bit) {
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
       }
       // Of the elements equal to it the lowest tokens are wanted: those below the least `end` that makes k.
       int end = lo;
-      for (int step = 1 << 15; step > 0; step >>= 1) {  // a piece holds at most 2^15 elements
+      for (int step = 1 << 15; step > 0; step >>= 1) {  // a round holds at most 2^15 elements
         int count = 0;
         for (int i = lo + tid; i < hi; i += kThreads) {
           const uint32_t o = ordered(to_float(x[i]));
@@ -341,26 +343,54 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
         }
         if (block_sum<kWarps>(count, s_i) < k) end += step;
       }
-      if (tid == 0) s_n = 0;
-      __syncthreads();
       for (int i = lo + tid; i < hi; i += kThreads) {
         const uint32_t o = ordered(to_float(x[i]));
-        if (o > key || (o == key && i <= end)) list[atomicAdd(&s_n, 1)] = rank_key(o, i);
+        if (o > key || (o == key && i <= end)) list[atomicAdd(&s_listed, 1)] = rank_key(o, i);
       }
       __syncthreads();
-      n = s_n;
     }
+    int n = s_listed;
     if (round > 0) {
       for (int i = tid; i < k; i += kThreads) list[n + i] = best[i];
       n += k;
     }
     if (tid < 8) list[n + tid] = 0;
     __syncthreads();
+    if (tid == 0) s_n = s_listed = 0;
     for (int i = tid; i < n; i += kThreads) {
       const unsigned long long own = list[i];
       const int before = larger(list, n, own);
       if (before < k && own != 0) best[before] = own;
     }
+    __syncthreads();
+    pending = 0;
+    // what comes later has to reach the k-th largest so far; a NaN there stays out of the comparison
+    if (best[k - 1] != 0) bound = fmaxf(bound, unordered((uint32_t)(best[k - 1] >> 32)));
+  }
+
+  // the block's sums, against its largest reference
+  Sums sums;
+  {
+    float x = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    if (lane == 0) s_a[warp] = x;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) x = fmaxf(x, s_a[w]);
+    const float shift = x == -INFINITY ? 0.f : (m - x) * FTA_LOG2E - r, f = fta_exp2(shift);
+    t = f == 0.f ? 0.f : f * (t + shift * s);
+    s *= f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (lane == 0) { s_b[warp] = s; s_c[warp] = t; }
+    __syncthreads();
+    sums = Sums{x, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) { sums.s += s_b[w]; sums.t += s_c[w]; }
   }
 
   // the row's blocks join in the first one
@@ -381,7 +411,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     if (tid < 8) list[k + tid] = 0;
     __syncthreads();
   }
-  const float m = sums.m, s = sums.s;
+  m = sums.m;
+  s = sums.s;
   const float log2_s = fta_log2(s);
   const float log_s = log2_s * FTA_LN2;
   if (tid == 0) {
@@ -409,8 +440,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
 
 int pieces_of(const FtaLogprobParams& p) {
   const int ve = p.dtype == FTA_DTYPE_F32 ? 4 : 8;
-  // a row's start may push its elements up to ve - 1 places into the chunks
-  return fta_cdiv(p.vocab + ve - 1, kThreads * kChunks * ve);
+  return p.vocab < ve ? 1 : fta_cdiv(p.vocab / ve, kThreads * kChunks);
 }
 
 template <typename T>

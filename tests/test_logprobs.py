@@ -1,9 +1,10 @@
 """Log probabilities of given tokens (token_logprobs) against a plain statement in 64 bits, and its refusals.
 
 Tolerances.  A term e^(x - m) is off by 2^-22 (the exponential) and |x - m| 2^-23 of itself; a sum of
-terms of one sign by at most the number of additions on one path, 64 in a thread, then 5 + 16 + 64
-joins, times 2^-24: below 10^-5 together for the logarithm of the sum, and 10^-5 of t / s, which is at
-most the entropy plus log s.  The result's own rounding is 2^-24 of it.  Tokens are exact."""
+terms of one sign by at most the number of additions on one path (8 in a chunk, a chunk a time in a
+thread, at most 8 rounds of 8 here, then 5 + 8 + 8 joins) times 2^-24, and each of at most 4 moves of the
+reference by 2^-22: below 10^-5 together for the logarithm of the sum, and 10^-5 of t / s, which is at most
+the entropy plus log s.  The result's own rounding is 2^-24 of it.  Tokens are exact."""
 import ctypes as C
 
 import pytest
