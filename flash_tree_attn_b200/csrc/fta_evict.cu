@@ -1,11 +1,14 @@
 // Eviction of cache rows by accumulated attention weight (include/fta.h: fta_evict_rows).
 //
 // Select: one block per (sequence, KV head) finds the smallest weight that is kept by a radix select
-// over the weights' ordered bits (four passes of 8 bits), then walks the rows once more in order and
-// writes the list of kept rows, moving their weights up as it goes.
+// over the weights' ordered bits, held in shared memory, counts the kept rows of each warp's stretch, and
+// writes the list of kept rows and their weights in order.  Digits are 11, 11 and 10 bits wide: the top
+// 11 are the exponent and two bits more, over which weights spread; with 8 bits most of a warp's
+// counts met in the same few bins, one after the other.
 // Move: new row i takes old row kept[i] >= i.  A block owns a column slice of one head's K or V and
 // walks the list in chunks: all of a chunk's rows are read, then written.  A write goes to rows below
-// the chunk's end, a later chunk's rows lie at or above it, so reads never see a write.
+// the chunk's end, a later chunk's rows lie at or above it, so reads never see a write, and the next
+// chunk's reads are under way while this one's rows are written.
 //
 // What bounds it: the kept rows of K and V are read and written once (8 D bytes a row); the weights
 // are small against that.
@@ -14,8 +17,10 @@
 namespace {
 
 constexpr int kSelect = 1024;
+constexpr int kKeys = 24 * 1024;  // rows whose weights fit the select block's shared memory (two blocks an SM)
 constexpr int kMove = 256;
-constexpr int kAhead = 4;  // rows in flight per thread
+constexpr int kAhead = 3;         // rows per thread and chunk
+constexpr int kBins = 2048;
 
 // order of floats as unsigned integers; -0 and +0 alike, NaN on top
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -25,12 +30,33 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictParams p) {
-  __shared__ int hist[256];
+// Moves w[from, from + n) to w[to, to + n), to <= from: a chunk is read, then written.
+template <typename F> __device__ __forceinline__ void move_up(float* w, int to, int n, F&& from) {
+  for (int base = 0; base < n; base += 4 * kSelect) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + u * kSelect + (int)threadIdx.x;
+      x[u] = i < n ? w[from(i)] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + u * kSelect + (int)threadIdx.x;
+      if (i < n) w[to + i] = x[u];
+    }
+  }
+}
+
+// `room`: weights that the dynamic shared memory holds; a longer sequence's are read again in every pass
+__global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictParams p, const int room) {
+  extern __shared__ float s_w[];
+  __shared__ int hist[kBins];
   __shared__ int s_bin, s_left;
-  __shared__ int s_warp[2][32];
+  __shared__ int s_equal[32], s_larger[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the move's blocks wait for this grid's end
   const int L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx);
   int* kept = p.kept + (long long)blockIdx.x * p.budget;
   if (L <= p.budget) {
@@ -40,134 +66,157 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictPar
   float* w = p.row_weights + b * p.rw_sb + h * p.rw_sh;
   const int n = L - p.recent, want = p.budget - p.recent;  // n > want
 
-  // the want-th largest of w[0, n): its bits from the top, `left` counts down to its rank among equals
-  uint32_t prefix = 0, mask = 0;
-  int left = want;
   if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelect) hist[i] = 0;
+    const bool held = n <= room;
+    if (held)
+      for (int r = tid; r < n; r += kSelect) s_w[r] = w[r];
+    auto key = [&](int r) { return ordered(held ? s_w[r] : w[r]); };
+
+    // the want-th largest of w[0, n): its bits from the top, `left` counts down to its rank among equals
+    uint32_t prefix = 0, mask = 0;
+    int left = want;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, digit = pass < 2 ? 2047 : 1023;
+      hist[tid] = 0;
+      hist[tid + kSelect] = 0;
       __syncthreads();
       for (int r = tid; r < n; r += kSelect) {
-        const uint32_t k = ordered(w[r]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+        const uint32_t k = key(r);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit], 1);
       }
       __syncthreads();
-      if (warp == 0) {  // lane holds bins 8 lane .. 8 lane + 7; bins above it come first
-        int mine = 0;
+      // a thread holds bins 2047 - 2 tid and the one below; `above` counts the bins that come before
+      const int bin = kBins - 1 - 2 * tid, first = hist[bin], mine = first + hist[bin - 1];
+      int above = mine;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mine += hist[8 * lane + i];
-        int above = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int t = __shfl_down_sync(0xffffffffu, above, o);
-          if (lane + o < 32) above += t;
-        }
-        above -= mine;
-        if (above < left && left <= above + mine) {
-          int rest = left - above, i = 7;
-          while (rest > hist[8 * lane + i]) rest -= hist[8 * lane + i--];
-          s_bin = 8 * lane + i;
-          s_left = rest;
-        }
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, above, o);
+        if (lane >= o) above += t;
+      }
+      if (lane == 31) s_equal[warp] = above;
+      __syncthreads();
+      above += __reduce_add_sync(0xffffffffu, lane < warp ? s_equal[lane] : 0) - mine;
+      if (above < left && left <= above + mine) {
+        const bool upper = left <= above + first;
+        s_bin = upper ? bin : bin - 1;
+        s_left = left - above - (upper ? 0 : first);
       }
       __syncthreads();
       prefix |= (uint32_t)s_bin << shift;
-      mask |= 255u << shift;
+      mask |= (uint32_t)digit << shift;
       left = s_left;
-      __syncthreads();
     }
-  }
 
-  // in order: larger ones, and the first `left` equal ones
-  int taken = 0, equal = 0;  // kept so far, equal ones seen so far
-  for (int base = 0; base < n && want > 0; base += kSelect) {
-    const int r = base + tid;
-    const float x = r < n ? w[r] : 0.f;
-    const uint32_t k = ordered(x);
-    const bool eq = r < n && k == prefix, gt = r < n && k > prefix;
-    const unsigned eqs = __ballot_sync(0xffffffffu, eq), gts = __ballot_sync(0xffffffffu, gt);
-    if (lane == 0) { s_warp[0][warp] = __popc(eqs); s_warp[1][warp] = __popc(gts); }
-    __syncthreads();
-    int e = s_warp[0][lane], g = s_warp[1][lane];  // 32 warps: inclusive sums over them
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int te = __shfl_up_sync(0xffffffffu, e, o), tg = __shfl_up_sync(0xffffffffu, g, o);
-      if (lane >= o) { e += te; g += tg; }
+    // Larger ones are kept, and the first `left` equal ones.  Each warp counts both in a stretch of rows,
+    // then, knowing what lies before it, writes its part of the list.
+    const int per = fta_cdiv(fta_cdiv(n, 32), 32) * 32, r0 = min(n, warp * per), r1 = min(n, r0 + per);
+    int equal = 0, larger = 0;
+    for (int r = r0 + lane; r - lane < r1; r += 32) {
+      const uint32_t k = r < r1 ? key(r) : 0u;  // 0: below every weight
+      equal += __popc(__ballot_sync(0xffffffffu, k == prefix));
+      larger += __popc(__ballot_sync(0xffffffffu, k > prefix));
     }
-    const int e_all = __shfl_sync(0xffffffffu, e, 31), g_all = __shfl_sync(0xffffffffu, g, 31);
-    const int e_before = warp == 0 ? 0 : __shfl_sync(0xffffffffu, e, (warp - 1) & 31);
-    const int g_before = warp == 0 ? 0 : __shfl_sync(0xffffffffu, g, (warp - 1) & 31);
-    const unsigned below = (1u << lane) - 1;
-    const int my_eq = equal + e_before + __popc(eqs & below);  // equal ones before this row
-    const int my_gt = g_before + __popc(gts & below);
-    if (gt || (eq && my_eq < left)) {
-      const int at = taken + my_gt + min(my_eq, left) - min(equal, left);
-      kept[at] = r;
-      w[at] = x;  // at <= r, and every row of this chunk has been read
-    }
-    taken += g_all + min(equal + e_all, left) - min(equal, left);
-    equal += e_all;
+    __syncthreads();  // s_equal of the last pass has been read
+    if (lane == 0) { s_equal[warp] = equal; s_larger[warp] = larger; }
     __syncthreads();
+    equal = __reduce_add_sync(0xffffffffu, lane < warp ? s_equal[lane] : 0);
+    larger = __reduce_add_sync(0xffffffffu, lane < warp ? s_larger[lane] : 0);
+    for (int r = r0 + lane; r - lane < r1; r += 32) {
+      const uint32_t k = r < r1 ? key(r) : 0u;
+      const unsigned eqs = __ballot_sync(0xffffffffu, k == prefix), gts = __ballot_sync(0xffffffffu, k > prefix);
+      const unsigned below = (1u << lane) - 1;
+      const int e = equal + __popc(eqs & below);  // equal ones before this row
+      if (k > prefix || (k == prefix && e < left)) {
+        const int at = larger + __popc(gts & below) + min(e, left);
+        kept[at] = r;
+        if (held) w[at] = s_w[r];  // nobody reads w[0, n) any more
+      }
+      equal += __popc(eqs);
+      larger += __popc(gts);
+    }
+    __syncthreads();
+    if (!held) move_up(w, 0, want, [&](int i) { return kept[i]; });
   }
-  // the recent rows move up behind them
-  for (int base = 0; base < p.recent; base += kSelect) {
-    const int i = base + tid;
-    const float x = i < p.recent ? w[n + i] : 0.f;
-    __syncthreads();
-    if (i < p.recent) {
-      kept[want + i] = n + i;
-      w[want + i] = x;
-    }
-  }
+  for (int i = tid; i < p.recent; i += kSelect) kept[want + i] = n + i;
+  move_up(w, want, p.recent, [&](int i) { return n + i; });
   __syncthreads();
   for (int r = p.budget + tid; r < L; r += kSelect) w[r] = 0.f;
 }
 
 // grid = (B * Hkv, K or V, column slices); a row of a slice is `chunks` 16-byte chunks
-__global__ void __launch_bounds__(kMove) evict_move_kernel(const FtaEvictParams p, const int chunks) {
+__global__ void __launch_bounds__(kMove, 4) evict_move_kernel(const FtaEvictParams p, const int chunks) {
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
   const int* kept = p.kept + (long long)blockIdx.x * p.budget;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (blockIdx.y == 0 && blockIdx.z == 0 && h == 0 && threadIdx.x == 0) {
     // the select kernel has read the lengths, and this one does not
     const int L = min(fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx), p.budget);
     if (p.len_is_i64) reinterpret_cast<long long*>(p.kv_seq_len)[b] = L;
     else reinterpret_cast<int*>(p.kv_seq_len)[b] = L;
   }
-  // kept[i] - i never falls: rows before the first moved one stay where they are
+  // kept[i] - i never falls: rows before the first moved one stay where they are.  Each step of the search
+  // probes kMove places at once.
   int lo = 0, hi = p.budget;
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    const int r = kept[mid];
-    if (r > mid) hi = mid; else lo = mid + 1;
+    const int step = fta_cdiv(hi - lo, kMove), i = lo + (int)threadIdx.x * step;
+    const int stay = __syncthreads_count(i < hi && kept[i] <= i);  // probes 0 .. stay - 1 stay
+    if (stay == 0) break;  // lo itself moves
+    const int from = lo + (stay - 1) * step + 1;
+    hi = min(hi, from - 1 + step);  // the next probe moves, or lies at the end
+    lo = from;
   }
   const long long sb = blockIdx.y ? p.v_sb : p.k_sb, sh = blockIdx.y ? p.v_sh : p.k_sh, st = blockIdx.y ? p.v_st : p.k_st;
-  uint16_t* cache = (uint16_t*)(blockIdx.y ? p.v_cache : p.k_cache) + h * sh + (long long)blockIdx.z * chunks * 8;
+  const int per = kMove / chunks, mine = threadIdx.x / chunks, c = threadIdx.x - mine * chunks;
+  uint16_t* cache = (uint16_t*)(blockIdx.y ? p.v_cache : p.k_cache) + h * sh + ((long long)blockIdx.z * chunks + c) * 8;
+  const int page_bits = (p.page_size & (p.page_size - 1)) == 0 ? __ffs(p.page_size) - 1 : -1;  // a division costs as much as a row's copy
+  const int* table = p.block_table + b * p.bt_sb;
   auto row_at = [&](int r) -> uint4* {
     long long at = b;
     if (p.block_table != nullptr) {
-      at = p.block_table[b * p.bt_sb + r / p.page_size];
+      const int slot = page_bits >= 0 ? r >> page_bits : r / p.page_size;
+      at = table[slot];
       if (at < 0 || at >= p.n_pages) return nullptr;
-      r %= p.page_size;
+      r -= slot * p.page_size;
     }
     return reinterpret_cast<uint4*>(cache + at * sb + (long long)r * st);
   };
-  const int per = kMove / chunks, mine = threadIdx.x / chunks, c = threadIdx.x - mine * chunks;
-  for (int base = lo; base < p.budget; base += per * kAhead) {
-    uint4 x[kAhead];
-    bool got[kAhead];
+  // three stages: which rows (two chunks ahead), their contents (one ahead), the writes
+  int rows[kAhead];
+  uint4 now[kAhead], next[kAhead];
+  unsigned has_now = 0, has_next = 0;
+  auto ask = [&](int base) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = base + u * per + mine;
-      const uint4* src = i < p.budget && kept[i] >= 0 ? row_at(kept[i]) : nullptr;
-      got[u] = src != nullptr;
-      if (got[u]) x[u] = src[c];
+      rows[u] = i < p.budget ? kept[i] : -1;
     }
-    __syncthreads();
+  };
+  auto read = [&](uint4 (&x)[kAhead]) {
+    unsigned has = 0;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      uint4* dst = got[u] ? row_at(base + u * per + mine) : nullptr;
-      if (dst != nullptr) dst[c] = x[u];
+      const uint4* src = rows[u] >= 0 ? row_at(rows[u]) : nullptr;
+      if (src != nullptr) { x[u] = *src; has |= 1u << u; }
     }
+    return has;
+  };
+  const int chunk = per * kAhead;
+  if (lo >= p.budget) return;
+  ask(lo);
+  has_now = read(now);
+  ask(lo + chunk);
+  for (int base = lo; base < p.budget; base += chunk) {
+    has_next = read(next);
+    ask(base + 2 * chunk);
+    __syncthreads();  // everybody has read this chunk
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      uint4* dst = (has_now >> u) & 1 ? row_at(base + u * per + mine) : nullptr;
+      if (dst != nullptr) *dst = now[u];
+      now[u] = next[u];
+    }
+    has_now = has_next;
   }
 }
 
@@ -185,11 +234,28 @@ extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
   if (p->block_table && (p->page_size < 1 || p->n_pages < 1 || p->bt_sb < 0 || (p->B > 1 && (long long)p->bt_sb * p->page_size < p->ctx)))
     return FTA_E_BADARG;
   cudaStream_t st = (cudaStream_t)stream;
-  evict_select_kernel<<<p->B * p->Hkv, kSelect, 0, st>>>(*p);
+  static unsigned long long configured = 0ull;  // per device: the opt-in shared-memory limit is set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return fta_cuda_fail(e);
+  if (!((configured >> (dev & 63)) & 1ull)) {
+    e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeys * 4);
+    if (e != cudaSuccess) return fta_cuda_fail(e);
+    configured |= 1ull << (dev & 63);
+  }
+  const int room = p->ctx < kKeys ? p->ctx : kKeys;
+  evict_select_kernel<<<p->B * p->Hkv, kSelect, room * 4, st>>>(*p, room);
   // column slices until there are blocks for every SM; no slice below a 32-byte sector
   int slices = 1;
   while ((long long)p->B * p->Hkv * 2 * slices < 2 * 148 && p->D / 8 / slices > 2) slices *= 2;
-  evict_move_kernel<<<dim3(p->B * p->Hkv, 2, slices), kMove, 0, st>>>(*p, p->D / 8 / slices);
-  const cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return fta_cuda_fail(e);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p->B * p->Hkv, 2, slices); cfg.blockDim = dim3(kMove); cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, *p, p->D / 8 / slices);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
