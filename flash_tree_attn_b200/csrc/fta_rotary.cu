@@ -7,7 +7,8 @@
 // half-turns, go to sincospi.
 //
 // What bounds it: each element is read once and written once; nothing else moves but 8 bytes per
-// pair.  A block works out the cosines and sines of its tokens once, in shared memory, for all heads.
+// pair.  A block works out the cosines and sines of its tokens once, in shared memory, for all heads, while
+// the first of the heads' elements are on their way.
 #include "fta_common.cuh"
 
 namespace {
@@ -26,27 +27,77 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const float (&f)[8]
   return make_uint4(FtaType<T>::pack(f[0], f[1]), FtaType<T>::pack(f[2], f[3]), FtaType<T>::pack(f[4], f[5]), FtaType<T>::pack(f[6], f[7]));
 }
 
-// grid = (token, sequence).  A head row is D / 16 lane tasks of two 16-byte chunks: the two halves of 8
-// pairs (or 8 adjacent pairs), or 16 elements that are only copied.
-template <typename T, bool APPEND>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const FtaRotaryParams p) {
-  __shared__ float2 cs[128];
-  const int i = blockIdx.x, b = blockIdx.y;
+// grid = (TOK tokens, sequence).  A head row is D / 16 lane tasks of two 16-byte chunks, neighbouring
+// lanes taking neighbouring chunks: the two halves of 8 pairs (half), twice 4 pairs (interleaved), or
+// elements that are only copied.  A head's rows of neighbouring tokens lie side by side in q, k and v.
+template <typename T, bool APPEND, int TOK>
+__global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const FtaRotaryParams p, const int row_bits) {
+  __shared__ float2 cs[TOK][128];
+  __shared__ long long s_dst[2][TOK];  // where the tokens' cache rows start (K, V); -1: nowhere
+  const int b = blockIdx.y, i0 = blockIdx.x * TOK;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // only the lengths' growth is launched to wait
+
+  const int rot16 = p.n_freq / 8;  // lane tasks of a row that turn (half); 1 << row_bits tasks in all
+  const int heads = p.H + p.Hkv + (APPEND ? p.Hkv : 0);
+  const bool half = p.layout == FTA_ROTARY_HALF;
+  // element offsets of task t's two chunks
+  auto chunks = [&](int t, int& x0, int& x1) {
+    if (half && t < rot16) {
+      x0 = 8 * t;
+      x1 = p.n_freq + 8 * t;
+    } else {
+      const int base = half ? 2 * p.n_freq : 0, u = half ? t - rot16 : t;
+      x0 = base + 8 * u;
+      x1 = x0 + (half ? p.D / 2 - p.n_freq : p.D / 2);
+    }
+  };
+  // task -> head row hh (queries, then keys, then values), token and lane task
+  const int tasks = (heads * TOK) << row_bits;
+  uint4 a, c;
+  auto read = [&](int task) {
+    const int row = task >> row_bits, i = i0 + row % TOK;
+    int hh = row / TOK;
+    if (task >= tasks || i >= p.Q) return;
+    int x0, x1;
+    chunks(task & ((1 << row_bits) - 1), x0, x1);
+    const T* src;
+    if (hh < p.H) src = (const T*)p.q + b * p.q_sb + hh * p.q_sh + i * p.q_sq;
+    else if ((hh -= p.H) < p.Hkv) src = (const T*)p.k + b * p.k_sb + hh * p.k_sh + i * p.k_sq;
+    else src = (const T*)p.v + b * p.v_sb + (hh - p.Hkv) * p.v_sh + i * p.v_sq;
+    a = *reinterpret_cast<const uint4*>(src + x0);
+    c = *reinterpret_cast<const uint4*>(src + x1);
+  };
+  read(threadIdx.x);
+
   const int L = APPEND ? fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx) : 0;
-  if ((int)threadIdx.x < p.n_freq) {
+  if (APPEND && (int)threadIdx.x < TOK) {
+    const int row = L + i0 + (int)threadIdx.x;
+    long long at = b, in = row;
+    bool fits = row >= 0 && row < p.ctx;
+    if (p.block_table != nullptr && fits) {
+      at = p.block_table[b * p.bt_sb + row / p.page_size];
+      in = row % p.page_size;
+      fits = at >= 0 && at < p.n_pages;
+    }
+    s_dst[0][threadIdx.x] = fits ? at * p.kc_sb + in * p.kc_st : -1;
+    s_dst[1][threadIdx.x] = fits ? at * p.vc_sb + in * p.vc_st : -1;
+  }
+  for (int j = threadIdx.x; j < p.n_freq * TOK; j += kThreads) {
+    const int tok = j / p.n_freq, f = j - tok * p.n_freq, i = i0 + tok;
+    if (i >= p.Q) break;
     long long pos = APPEND ? L : 0;
     if (p.positions != nullptr) {
       const long long at = b * p.pos_sb + i * p.pos_sq;
       pos = p.pos_is_i64 ? reinterpret_cast<const long long*>(p.positions)[at] : reinterpret_cast<const int*>(p.positions)[at];
     }
     pos += p.offsets != nullptr ? p.offsets[i] : (p.positions == nullptr || p.pos_sq == 0 ? i : 0);
-    const double turns = p.inv_freq[threadIdx.x] * 0.15915494309189535;  // 1 / (2 pi)
+    const double turns = p.inv_freq[f] * 0.15915494309189535;  // 1 / (2 pi)
     const unsigned long long step = __double2ull_rn((turns - floor(turns)) * 18446744073709551616.0);
     unsigned long long phase = (unsigned long long)pos * step;
     if (p.inverse) phase = 0ull - phase;
-    float s, c;
-    sincospif((float)(int)(phase >> 32) * 4.656612873077393e-10f, &s, &c);  // 2^-31: half-turns
-    cs[threadIdx.x] = make_float2(c * p.amplitude, s * p.amplitude);
+    float sn, cn;
+    sincospif((float)(int)(phase >> 32) * 4.656612873077393e-10f, &sn, &cn);  // 2^-31: half-turns
+    cs[tok][f] = make_float2(cn * p.amplitude, sn * p.amplitude);
   }
   // one block per sequence: nobody else reads the length, and everybody here has
   __syncthreads();
@@ -56,69 +107,55 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const FtaRotaryParams 
     else reinterpret_cast<int*>(p.kv_seq_len)[b] = to;
   }
 
-  const int per_row = p.D / 16, rot16 = p.n_freq / 8;  // lane tasks of a row, those that turn
-  const int heads = p.H + p.Hkv + (APPEND ? p.Hkv : 0);
-  long long kdst = 0, vdst = 0;  // where the cache row starts
-  bool fits = true;
-  if (APPEND) {
-    const int row = L + i;
-    long long at = b, r = row;
-    fits = row >= 0 && row < p.ctx;
-    if (p.block_table != nullptr && fits) {
-      at = p.block_table[b * p.bt_sb + row / p.page_size];
-      r = row % p.page_size;
-      fits = at >= 0 && at < p.n_pages;
-    }
-    kdst = at * p.kc_sb + r * p.kc_st;
-    vdst = at * p.vc_sb + r * p.vc_st;
-  }
-  for (int task = threadIdx.x; task < heads * per_row; task += kThreads) {
-    const int hh = task / per_row, t = task - hh * per_row;
-    const T* src;
-    T* dst;
-    bool turn = t < rot16;
-    if (hh < p.H) {
-      src = (const T*)p.q + b * p.q_sb + hh * p.q_sh + i * p.q_sq;
-      dst = (T*)p.q_out + (((long long)b * p.H + hh) * p.Q + i) * p.D;
-    } else if (hh < p.H + p.Hkv) {
-      const int h = hh - p.H;
-      src = (const T*)p.k + b * p.k_sb + h * p.k_sh + i * p.k_sq;
-      dst = APPEND ? (T*)p.k_cache + kdst + h * p.kc_sh : (T*)p.k_out + (((long long)b * p.Hkv + h) * p.Q + i) * p.D;
-      if (!fits) continue;
-    } else {
-      const int h = hh - p.H - p.Hkv;
-      src = (const T*)p.v + b * p.v_sb + h * p.v_sh + i * p.v_sq;
-      dst = (T*)p.v_cache + vdst + h * p.vc_sh;
-      turn = false;
-      if (!fits) continue;
-    }
-    const bool halves = p.layout == FTA_ROTARY_HALF && t < rot16;  // v included: the same chunks, copied
-    const int x0 = halves ? 8 * t : 16 * t, x1 = halves ? p.n_freq + 8 * t : 16 * t + 8;
-    uint4 a = *reinterpret_cast<const uint4*>(src + x0), c = *reinterpret_cast<const uint4*>(src + x1);
-    if (turn) {
-      float u[8], w[8];
-      unpack8<T>(a, u);
-      unpack8<T>(c, w);
-      if (p.layout == FTA_ROTARY_HALF) {
+  // eight blocks an SM keep enough rows in flight: two tasks a thread at once, with five blocks, took as long
+  for (int task = threadIdx.x; task < tasks; task += kThreads) {
+    if (task != (int)threadIdx.x) read(task);
+    const int row = task >> row_bits, t = task & ((1 << row_bits) - 1);
+    const int tok = row % TOK, i = i0 + tok, hh = row / TOK;
+    if (i >= p.Q) continue;
+    int x0, x1;
+    chunks(t, x0, x1);
+    if (hh < p.H + p.Hkv && (half ? t < rot16 : x0 < 2 * p.n_freq)) {
+      float y[8], z[8];
+      unpack8<T>(a, y);
+      unpack8<T>(c, z);
+      if (half) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float2 f = cs[8 * t + e];
-          const float y = u[e] * f.x - w[e] * f.y;
-          w[e] = w[e] * f.x + u[e] * f.y;
-          u[e] = y;
+          const float2 f = cs[tok][8 * t + e];
+          const float n = y[e] * f.x - z[e] * f.y;
+          z[e] = z[e] * f.x + y[e] * f.y;
+          y[e] = n;
         }
       } else {
+        const bool both = x1 < 2 * p.n_freq;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 f = cs[8 * t + e];
-          float* z = e < 4 ? u + 2 * e : w + 2 * (e - 4);
-          const float y = z[0] * f.x - z[1] * f.y;
-          z[1] = z[1] * f.x + z[0] * f.y;
-          z[0] = y;
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = cs[tok][x0 / 2 + e];
+          const float n = y[2 * e] * f.x - y[2 * e + 1] * f.y;
+          y[2 * e + 1] = y[2 * e + 1] * f.x + y[2 * e] * f.y;
+          y[2 * e] = n;
+          if (both) {
+            const float2 g = cs[tok][x1 / 2 + e];
+            const float n1 = z[2 * e] * g.x - z[2 * e + 1] * g.y;
+            z[2 * e + 1] = z[2 * e + 1] * g.x + z[2 * e] * g.y;
+            z[2 * e] = n1;
+          }
         }
       }
-      a = pack8<T>(u);
-      c = pack8<T>(w);
+      a = pack8<T>(y);
+      c = pack8<T>(z);
+    }
+    T* dst;
+    if (hh < p.H) {
+      dst = (T*)p.q_out + (((long long)b * p.H + hh) * p.Q + i) * p.D;
+    } else if (!APPEND) {
+      dst = (T*)p.k_out + (((long long)b * p.Hkv + hh - p.H) * p.Q + i) * p.D;
+    } else {
+      const bool v = hh >= p.H + p.Hkv;
+      const long long at = s_dst[v][tok];
+      if (at < 0) continue;
+      dst = v ? (T*)p.v_cache + at + (hh - p.H - p.Hkv) * p.vc_sh : (T*)p.k_cache + at + (hh - p.H) * p.kc_sh;
     }
     *reinterpret_cast<uint4*>(dst + x0) = a;
     *reinterpret_cast<uint4*>(dst + x1) = c;
@@ -127,6 +164,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const FtaRotaryParams 
 
 __global__ void grow_lengths_kernel(const FtaRotaryParams p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // every block of the append has read the lengths
   if (b >= p.B) return;
   const long long L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx) + (long long)p.Q;
   const int to = (int)(L < p.ctx ? L : p.ctx);
@@ -160,11 +198,26 @@ int check(const FtaRotaryParams* p, bool append) {
 template <bool APPEND>
 int launch(const FtaRotaryParams* p, cudaStream_t st) {
   if (int rc = check(p, APPEND)) return rc;
-  const dim3 grid(p->Q, p->B);
-  if (p->dtype == FTA_DTYPE_F16) rotary_kernel<__half, APPEND><<<grid, kThreads, 0, st>>>(*p);
-  else rotary_kernel<__nv_bfloat16, APPEND><<<grid, kThreads, 0, st>>>(*p);
-  if (APPEND && p->Q > 1) grow_lengths_kernel<<<(p->B + 127) / 128, 128, 0, st>>>(*p);
-  const cudaError_t e = cudaGetLastError();
+  // Four tokens a block once that still leaves every SM several blocks: they share the start of a block
+  // (length, page, a barrier) and a head's rows of four tokens are one piece of memory.
+  const bool four = (long long)p->B * p->Q >= 148 * 16;
+  const dim3 grid(four ? (p->Q + 3) / 4 : p->Q, p->B);
+  const int bits = p->D == 32 ? 1 : p->D == 64 ? 2 : p->D == 128 ? 3 : 4;
+  const bool f16 = p->dtype == FTA_DTYPE_F16;
+  if (four && f16) rotary_kernel<__half, APPEND, 4><<<grid, kThreads, 0, st>>>(*p, bits);
+  else if (four) rotary_kernel<__nv_bfloat16, APPEND, 4><<<grid, kThreads, 0, st>>>(*p, bits);
+  else if (f16) rotary_kernel<__half, APPEND, 1><<<grid, kThreads, 0, st>>>(*p, bits);
+  else rotary_kernel<__nv_bfloat16, APPEND, 1><<<grid, kThreads, 0, st>>>(*p, bits);
+  cudaError_t e = cudaGetLastError();
+  if (APPEND && grid.x > 1 && e == cudaSuccess) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((p->B + 127) / 128); cfg.blockDim = dim3(128); cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, grow_lengths_kernel, *p);
+  }
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
 

@@ -27,15 +27,16 @@ struct FtaTokenWs {  // byte offsets of the workspace's parts
 
 // part_o [2 * grid][R][D] and part_l [2 * grid][R] as in FtaParams' BALANCED workspace (LSEs in log2
 // units); desc [B * U] int2 {pieces, first group of blocks} per unit; with row weights also the log2
-// LSE of every head [B * H] and every score [B * H][ctx] in log2 units.
+// LSE of every head [B * H] and every score [B * H][ctx, padded to whole 16 bytes] in log2 units.
+__host__ __device__ __forceinline__ long long fta_token_pitch(int ctx) { return ((long long)ctx + 3) / 4 * 4; }
 __host__ __device__ __forceinline__ FtaTokenWs fta_token_ws(int grid, int R, int D, int B, int U, int H, int ctx, bool weights) {
   FtaTokenWs w;
   w.part_o = 0;
   w.part_l = w.part_o + 2ll * grid * R * D * 4;
   w.desc = w.part_l + 2ll * grid * R * 4;
   w.lse2 = w.desc + (long long)B * U * 8;
-  w.scores = w.lse2 + (weights ? (long long)B * H * 4 : 0);
-  w.bytes = w.scores + (weights ? (long long)B * H * ctx * 4 : 0);
+  w.scores = (w.lse2 + (weights ? (long long)B * H * 4 : 0) + 15) / 16 * 16;
+  w.bytes = w.scores + (weights ? (long long)B * H * fta_token_pitch(ctx) * 4 : 0);
   return w;
 }
 

@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__global__ void __launch_bounds__(kThreads) token_join_kernel(const FtaTokenParams p, const FtaGeom g, const int chunk_rows) {
+__global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenParams p, const FtaGeom g, const int chunk_rows) {
   __shared__ float s_lse[FTA_MAX_GROUP];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / p.Hkv, kvh = blockIdx.x - b * p.Hkv;
@@ -87,25 +87,35 @@ __global__ void __launch_bounds__(kThreads) token_join_kernel(const FtaTokenPara
   }
   if (!weights) return;
   __syncthreads();
-  const float* scores = reinterpret_cast<const float*>(wsb + ws.scores) + ((long long)b * p.H + kvh * G) * p.ctx;
+  // A thread has four consecutive rows and asks for eight heads' scores of them together: the loop waits
+  // for memory and for nothing else.
+  const long long pitch = fta_token_pitch(p.ctx);
+  const float* scores = reinterpret_cast<const float*>(wsb + ws.scores) + ((long long)b * p.H + kvh * G) * pitch;
   float* out = p.row_weights + b * p.rw_sb + kvh * p.rw_sh;
-  // four heads' scores of a row are asked for together: the loop waits for memory and for nothing else
-  const int first = max(row0, p.window > 0 ? L - p.window : 0), end = min(L, row0 + chunk_rows);
-  for (int row = first + threadIdx.x; row < end; row += kThreads) {
-    float w = 0.f;
-    const float old = out[row];
-    for (int h0 = 0; h0 < G; h0 += 4) {
-      float x[4];
+  const int first = p.window > 0 ? max(0, L - p.window) : 0;
+  const int row = row0 + 4 * (int)threadIdx.x;
+  if (row + 3 < first || row >= L) return;
+  float old[4], w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = h0 + u < G ? __ldcs(scores + (long long)(h0 + u) * p.ctx + row) : -INFINITY;
+  for (int e = 0; e < 4; ++e) old[e] = row + e >= first && row + e < L ? out[row + e] : 0.f;
+  for (int h0 = 0; h0 < G; h0 += 8) {
+    float4 x[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float total = h0 + u < G ? s_lse[h0 + u] : 0.f;
-        w += total == -INFINITY ? 0.f : fta_exp2(x[u] - total);
-      }
+    for (int u = 0; u < 8; ++u)
+      if (h0 + u < G) x[u] = __ldcs(reinterpret_cast<const float4*>(scores + (h0 + u) * pitch + row));
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float total = h0 + u < G ? s_lse[h0 + u] : -INFINITY;
+      if (total == -INFINITY) continue;
+      w[0] += fta_exp2(x[u].x - total);
+      w[1] += fta_exp2(x[u].y - total);
+      w[2] += fta_exp2(x[u].z - total);
+      w[3] += fta_exp2(x[u].w - total);
     }
-    out[row] = old + w;
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (row + e >= first && row + e < L) out[row + e] = old[e] + w[e];
 }
 
 template <typename F>
@@ -203,7 +213,7 @@ extern "C" int fta_decode_token(const FtaTokenParams* p, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e = (cudaError_t)token_variant(*p, [&](auto launch) { return (int)launch(*p, g, st, 0, nullptr); });
   if (e != cudaSuccess) return fta_cuda_fail(e);
-  const int chunk = 1024;  // 4 rows a thread: 256, 512 and 1024 rows a block took 136, 128 and 127 us on 131072 rows of 64 heads
+  const int chunk = 4 * kThreads;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -257,7 +257,7 @@ def test_c_entry_sizes(fta_lib):
     assert fta_lib.fta_decode_token(None, None) == _lib.FTA_E_BADARG
     plain, kept = _fake(), _fake(row_weights=4096)
     a, b = (fta_lib.fta_decode_token_workspace_bytes(C.byref(x)) for x in (plain, kept))
-    assert a > 0 and b == a + 4 * 2 * 8 * (1 + 256)  # an LSE and ctx scores per head
+    assert a > 0 and 0 <= b - a - 4 * 2 * 8 * (1 + 256) < 16  # an LSE and ctx scores per head, aligned
     assert fta_lib.fta_decode_token_workspace_bytes(C.byref(_fake(D=48))) == -_lib.FTA_E_BADARG
 
 
