@@ -21,7 +21,13 @@ from .op import (  # noqa: F401
 from .decode import decode_attention, decode_attention_paged, evict_rows  # noqa: F401,E402
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401,E402
 from .rotary import append_tokens, apply_rotary, rotary_frequencies  # noqa: F401,E402
-from .speculative import DraftTree, TreeVerifyAttention, accept_longest_path  # noqa: F401,E402
+from .speculative import (  # noqa: F401,E402
+    DraftTree,
+    TreeVerifyAttention,
+    accept_longest_path,
+    greedy_node_ok,
+    typical_node_ok,
+)
 
 __all__ = [
     "check_status",
@@ -37,6 +43,7 @@ __all__ = [
     "flash_decoding_attention",
     "flash_decoding_attention_paged",
     "flash_decoding_attention_with_lse",
+    "greedy_node_ok",
     "merge_partials",
     "prepare",
     "rotary_frequencies",
@@ -45,4 +52,5 @@ __all__ = [
     "set_grid_override",
     "token_logprobs",
     "TokenLogprobs",
+    "typical_node_ok",
 ]

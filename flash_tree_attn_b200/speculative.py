@@ -14,16 +14,25 @@ The reference stops at the operator and lists "integration into transformers, me
         idx, n = accept_longest_path(tree, node_ok)             # caller's acceptance rule -> a root path
         layer.commit(idx, n)                                    # accepted nodes' K/V join the cache
 
+A step without a draft is `layer.decode(q, k_new, v_new)`: the new token joins the cache and attends to
+it.  With `rotary` the layer turns queries and keys to their positions itself; with `track_weights` it
+adds up what every cache row was looked at, and `layer.evict(budget, recent)` keeps the cache within
+a budget by it.  `greedy_node_ok` and `typical_node_ok` are acceptance rules over the model's logits.
+
 Nothing here synchronises with the host: the lengths live on the device, the operator plans from
 them on the device, and `commit` updates them in place, so a whole step can sit in a CUDA graph.
 """
 from __future__ import annotations
 
+import math
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
+from .decode import decode_attention, decode_attention_paged, evict_rows
+from .logprobs import token_logprobs
 from .op import commit_accepted, flash_decoding_attention, flash_decoding_attention_paged
+from .rotary import append_tokens, apply_rotary
 
 
 class DraftTree:
@@ -56,6 +65,15 @@ class DraftTree:
         self.ancestors = anc.to(dev)                                   # [Q, Q] j is i or an ancestor of i
         self.paths = paths.to(dev)                                     # [Q, max_depth] root ... node, zero padded
         self.depth = torch.tensor(depth, dtype=torch.int32, device=dev)
+        children: List[List[int]] = [[] for _ in range(Q)]
+        slot = [0] * Q                                                 # which of its parent's children a node is
+        for i in range(1, Q):
+            slot[i] = len(children[parents[i]])
+            children[parents[i]].append(i)
+        fan = max(1, max(len(c) for c in children))
+        self.children = torch.tensor([c + [-1] * (fan - len(c)) for c in children], device=dev)  # [Q, fan], -1 padded
+        self.parent = torch.tensor([max(p, 0) for p in parents], device=dev)                     # the root's: itself
+        self.slot = torch.tensor(slot, device=dev)
         self.mask = torch.where(self.ancestors, float(allowed), float("-inf")).to(torch.float32)
 
 
@@ -79,6 +97,32 @@ def accept_longest_path(tree: DraftTree, node_ok: torch.Tensor) -> Tuple[torch.T
     return tree.paths[best].contiguous(), n
 
 
+def greedy_node_ok(tree: DraftTree, logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+    """Greedy verification: a node is accepted if its token is the likeliest one at its parent (the lower
+    token of equals); the root, whose token the model has chosen already, always is.
+
+    logits [bsz, q_len, vocab] of the tree's nodes, tokens [bsz, q_len] int32/int64 drafted at them.
+    Returns node_ok [bsz, q_len] bool as `accept_longest_path` takes it."""
+    best = token_logprobs(logits, top_k=1).top_ids[..., 0]
+    ok = tokens == best[:, tree.parent]
+    ok[:, 0] = True
+    return ok
+
+
+def typical_node_ok(tree: DraftTree, logits: torch.Tensor, tokens: torch.Tensor, epsilon: float = 0.09, delta: float = 0.3) -> torch.Tensor:
+    """Typical acceptance: a node is accepted if the model gives its token, at its parent, a probability
+    above min(epsilon, delta * exp(-entropy)): an unlikely token passes where the model is unsure.
+
+    Arguments and result as greedy_node_ok."""
+    drafted = tokens[:, tree.children.clamp(min=0)]                    # [bsz, q_len, fan]
+    drafted = torch.where(tree.children < 0, torch.full_like(drafted, -1), drafted)
+    r = token_logprobs(logits, drafted)
+    bar = torch.minimum(torch.full_like(r.entropy, math.log(epsilon)), math.log(delta) - r.entropy)
+    ok = r.logprobs[:, tree.parent, tree.slot] > bar[:, tree.parent]
+    ok[:, 0] = True
+    return ok
+
+
 class TreeVerifyAttention(torch.nn.Module):
     """The attention of one decoder layer during tree verification, with its KV cache.
 
@@ -89,11 +133,20 @@ class TreeVerifyAttention(torch.nn.Module):
     shuffled order at construction.
 
     forward() is the verify step and leaves the cache untouched; commit() appends the accepted
-    nodes' keys and values (as given to the last forward) and grows kv_seq_len in place."""
+    nodes' keys and values (as given to the last forward) and grows kv_seq_len in place.  decode() is
+    the step of one token without a draft.  The row of a token that finds the cache full is dropped.
+
+    rotary: (inv_freq, layout, amplitude) as apply_rotary takes them (`rotary_frequencies` makes the
+    first and the last); queries and new keys are then turned to next_position and on, which counts
+    every token of a sequence, evicted ones too.  Keys given to load_prefix are turned already.
+    track_weights: keep row_weights [max_batch, num_kv_heads, rows] of decode(), which evict() goes by.
+    Rows that verification looked at gain nothing; `recent` is there to keep new rows until decode()
+    has looked at them."""
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, max_batch: int, max_seq_len: int,
                  dtype: torch.dtype = torch.float16, device="cuda", page_size: Optional[int] = None,
-                 sm_scale: Optional[float] = None, seed: int = 0):
+                 sm_scale: Optional[float] = None, seed: int = 0,
+                 rotary: Optional[Tuple[torch.Tensor, str, float]] = None, track_weights: bool = False):
         super().__init__()
         assert num_heads % num_kv_heads == 0
         self.H, self.Hkv, self.D = num_heads, num_kv_heads, head_dim
@@ -116,6 +169,12 @@ class TreeVerifyAttention(torch.nn.Module):
         self.register_buffer("v_cache", torch.zeros_like(k), persistent=False)
         self.register_buffer("kv_seq_len", torch.zeros(max_batch, dtype=torch.int32, device=dev), persistent=False)
         self.register_buffer("block_table", table, persistent=False)
+        self.register_buffer("next_position", torch.zeros(max_batch, dtype=torch.int64, device=dev), persistent=False)
+        self.register_buffer("inv_freq", None if rotary is None else rotary[0].to(dev), persistent=False)
+        self.layout, self.amplitude = ("half", 1.0) if rotary is None else (rotary[1], float(rotary[2]))
+        rows = max_seq_len if table is None else table.size(1) * page_size
+        weights = torch.zeros((max_batch, num_kv_heads, rows), dtype=torch.float32, device=dev) if track_weights else None
+        self.register_buffer("row_weights", weights, persistent=False)
         self._last_kv = None
 
     @torch.no_grad()
@@ -135,13 +194,22 @@ class TreeVerifyAttention(torch.nn.Module):
                     self.k_cache[pg, :, : r1 - r0] = k[b, :, r0:r1]
                     self.v_cache[pg, :, : r1 - r0] = v[b, :, r0:r1]
         self.kv_seq_len[:B] = torch.as_tensor(list(lens), dtype=torch.int32)
+        self.next_position[:B] = torch.as_tensor(list(lens), dtype=torch.int64)
+        if self.row_weights is not None:
+            self.row_weights[:B] = 0.0
 
     @torch.no_grad()
-    def forward(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
+    def forward(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, mask: torch.Tensor,
+                depth: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Verify: q [bsz, num_heads, q_len, head_dim], k_new / v_new [bsz, num_kv_heads, q_len, head_dim]
-        of the draft tree's nodes, additive mask over the nodes.  Returns [bsz, num_heads, q_len, head_dim]."""
+        of the draft tree's nodes, additive mask over the nodes.  With rotary, depth [q_len] int32 says how
+        far each node lies behind next_position (`DraftTree.depth`).  Returns [bsz, num_heads, q_len, head_dim]."""
         B = q.size(0)
         lens = self.kv_seq_len[:B]
+        if self.inv_freq is not None:
+            assert depth is not None, "a layer with rotary positions needs the nodes' depths"
+            q, k_new = apply_rotary(q, k_new, self.next_position[:B], self.inv_freq, offsets=depth, layout=self.layout,
+                                    amplitude=self.amplitude)
         self._last_kv = (k_new, v_new)
         if self.block_table is None:
             return flash_decoding_attention(q, self.k_cache[:B], self.v_cache[:B], k_new, v_new, mask, lens, 64,
@@ -162,6 +230,35 @@ class TreeVerifyAttention(torch.nn.Module):
         else:
             commit_accepted(self.k_cache, self.v_cache, k_new, v_new, self.kv_seq_len[:B], accept_idx, accept_len,
                             kv_group_num=self.G, block_table=self.block_table[:B])
+        self.next_position[:B] += accept_len.to(self.next_position.device).clamp(0, accept_idx.size(1))
+
+    @torch.no_grad()
+    def decode(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
+        """One token without a draft: q [bsz, num_heads, 1, head_dim], k_new / v_new [bsz, num_kv_heads, 1,
+        head_dim].  The token joins the cache and attends to it, itself included.  Returns
+        [bsz, num_heads, 1, head_dim]."""
+        B = q.size(0)
+        assert q.size(2) == 1 and k_new.size(2) == 1, "decode() takes one new token per sequence"
+        lens, table = self.kv_seq_len[:B], None if self.block_table is None else self.block_table[:B]
+        k, v = (self.k_cache[:B], self.v_cache[:B]) if table is None else (self.k_cache, self.v_cache)
+        q = append_tokens(k, v, q, k_new, v_new, lens, inv_freq=self.inv_freq, layout=self.layout, amplitude=self.amplitude,
+                          positions=None if self.inv_freq is None else self.next_position[:B], block_table=table)
+        self.next_position[:B] += 1
+        opts = dict(max_seq_len_in_batch=self.max_seq_len, sm_scale=self.sm_scale, kv_group_num=self.G,
+                    row_weights=None if self.row_weights is None else self.row_weights[:B])
+        if table is None:
+            return decode_attention(q, k, v, lens, **opts)
+        return decode_attention_paged(q, k, v, table, lens, **opts)
+
+    @torch.no_grad()
+    def evict(self, budget: int, recent: int, batch: Optional[int] = None) -> torch.Tensor:
+        """Bring the first `batch` sequences (default: all) back to `budget` rows, the last `recent` of them
+        kept in any case (see evict_rows).  Returns the old row of every row, [bsz, num_kv_heads, budget]."""
+        assert self.row_weights is not None, "evict() needs a layer with track_weights"
+        B = self.kv_seq_len.size(0) if batch is None else int(batch)
+        table = None if self.block_table is None else self.block_table[:B]
+        k, v = (self.k_cache[:B], self.v_cache[:B]) if table is None else (self.k_cache, self.v_cache)
+        return evict_rows(k, v, self.kv_seq_len[:B], self.row_weights[:B], budget, recent, block_table=table)
 
 
 def reference_path_walk(parents: Sequence[int], ok_row: Sequence[bool]) -> List[int]:
