@@ -54,8 +54,9 @@ def check_caches(k: torch.Tensor, v: torch.Tensor, B: int, Hkv: int, D: int, dty
     return kr, vr, width * page, block_table.data_ptr(), stride, page, shape[0]
 
 
-def check_in_place(k: torch.Tensor, v: torch.Tensor, kv_seq_len: torch.Tensor, B: int) -> None:
-    assert not _overlaps(k) and not _overlaps(v), "caches are updated in place and must not be expanded"
+def check_in_place(k: torch.Tensor, v: torch.Tensor, kr, vr, kv_seq_len: torch.Tensor, B: int) -> None:
+    """kr, vr: the caches' pointers and strides."""
+    assert (0 not in kr or not _overlaps(k)) and (0 not in vr or not _overlaps(v)), "caches are updated in place and must not be expanded"
     assert B <= 1 or kv_seq_len.stride(0) == 1, "kv_seq_len is updated in place and must be contiguous"
 
 
@@ -113,11 +114,11 @@ def _decode(q, k, v, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, H, 1, D), dtype=dt, device=q.device)
     lse = torch.empty((B, H, 1), dtype=_f32, device=q.device) if return_lse else None
     if B and H:
-        size = _workspace(lib, dev, B, H, Hkv, D, ctx, code, weights, grid)
-        ws = out.new_empty(size)  # `size` elements of two bytes each
+        size = _workspace(lib, dev, B, H, Hkv, D, ctx, code, weights, window or 0, grid)
+        ws = out.new_empty(size) if size else None  # `size` elements of two bytes each
         launch(lib.fta_decode_token, pack_token(
             qr[0], qr[1], qr[2], *kr, *vr, kv_seq_len.data_ptr(), table, table_sb, slopes, out.data_ptr(), H * D, D,
-            lse.data_ptr() if return_lse else 0, H, rw, rw_sb, rw_sh, ws.data_ptr(), 2 * size,
+            lse.data_ptr() if return_lse else 0, H, rw, rw_sb, rw_sh, ws.data_ptr() if size else 0, 2 * size,
             1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), softcap or 0.0, window or 0, is64,
             B, H, Hkv, D, ctx, page, n_pages, code, grid, 0), dev, "fta_decode_token")
     return (out, lse) if return_lse else out
@@ -129,10 +130,10 @@ _ws_sizes = {}  # sizes -> 16-bit elements of workspace: a function of the sizes
 def _workspace(lib, *key) -> int:
     size = _ws_sizes.get(key)
     if size is None:
-        index, B, H, Hkv, D, ctx, code, weights, grid = key
+        index, B, H, Hkv, D, ctx, code, weights, window, grid = key
         p = _lib.FtaTokenParams()
         p.B, p.H, p.Hkv, p.D, p.ctx, p.dtype, p.grid_override = B, H, Hkv, D, ctx, code, grid
-        p.row_weights = 1 if weights else 0
+        p.row_weights, p.window = 1 if weights else 0, window
         with torch.cuda.device(index):
             size = lib.fta_decode_token_workspace_bytes(_lib.byref(p))
         if size < 0:
@@ -217,7 +218,7 @@ def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: i
     assert D in _HEAD_DIMS, "head_dim must be 32, 64, 128 or 256"
     kr, vr, ctx, table, table_sb, page, n_pages = check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
     is64 = check_lengths(kv_seq_len, B, dev)
-    check_in_place(k_cache, v_cache, kv_seq_len, B)
+    check_in_place(k_cache, v_cache, kr, vr, kv_seq_len, B)
     assert row_weights.dim() == 3, "row_weights must be [bsz, num_kv_heads, ctx]"
     rw, rw_sb, rw_sh = check_weights(row_weights, B, Hkv, ctx, dev)
     budget, recent = int(budget), int(recent)

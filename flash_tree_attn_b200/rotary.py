@@ -117,14 +117,14 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     assert code is not None and D in _HEAD_DIMS, "q must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
     n, layout = _check_frequencies(inv_freq, D, dev, layout)
     q, qr = _rows(q)
-    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    qo = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
     Hkv, kr, ko, kp = 0, (0, 0, 0, 0), None, 0
     if k is not None:
         assert k.dtype is dt and k.get_device() == dev and k.dim() == 4, "k must be of q's dtype and on its device"
         kb, Hkv, kq, kd = k.shape
         assert kb == B and kq == Q and kd == D, "k must be [bsz, num_kv_heads, q_len, head_dim]"
         k, kr = _rows(k)
-        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k) if k.is_contiguous() else torch.empty_like(k, memory_format=torch.contiguous_format)
         kp = ko.data_ptr()
     positions, pos, psb, psq, is64 = _check_positions(positions, B, Q, dev)
     off = 0
@@ -166,7 +166,7 @@ def append_tokens(k_cache, v_cache, q, k, v, kv_seq_len, *, inv_freq: Optional[t
     assert k.get_device() == dev and v.get_device() == dev and v.dtype is dt and v.shape == k.shape, "k and v must be alike, on the caches' device"
     kc, vc, ctx, table, table_sb, page, n_pages = check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
     len64 = check_lengths(kv_seq_len, B, dev)
-    check_in_place(k_cache, v_cache, kv_seq_len, B)
+    check_in_place(k_cache, v_cache, kc, vc, kv_seq_len, B)
     qb, H, qq, qd = q.shape
     assert qb == B and qq == Q and qd == D and q.dtype is dt and q.get_device() == dev, \
         "q must be [bsz, num_heads, q_len, head_dim] of k's dtype and on its device"
@@ -176,7 +176,7 @@ def append_tokens(k_cache, v_cache, q, k, v, kv_seq_len, *, inv_freq: Optional[t
     if inv_freq is not None:
         n, layout = _check_frequencies(inv_freq, D, dev, layout)
         q, qr = _rows(q)
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
         qo, freq = out.data_ptr(), inv_freq.data_ptr()
         if positions is not None:
             positions, pos, psb, psq, is64 = _check_positions(positions, B, Q, dev)

@@ -287,8 +287,8 @@ typedef struct FtaTokenParams {
   int32_t reserved_;
 } FtaTokenParams;
 
-/* Bytes of workspace the call needs on the current device; negative: -FTA_E_*.  Sizes, dtype,
-   grid_override and whether row_weights is NULL are read. */
+/* Bytes of workspace the call needs on the current device (0: none); negative: -FTA_E_*.  Sizes, window,
+   dtype, grid_override and whether row_weights is NULL are read. */
 int64_t fta_decode_token_workspace_bytes(const FtaTokenParams* p);
 int fta_decode_token(const FtaTokenParams* p, void* stream);
 

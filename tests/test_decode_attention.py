@@ -93,8 +93,12 @@ def test_matches_the_formula(dtype, case, grid):
     args = (q, k, v, lens, table, None, None, c["G"], opt.get("softcap"), slopes, opt.get("window"))
     out, lse = decode._decode(*args, w, True, grid=grid)
     _check(out, lse, w, ora, dtype, c["D"], opt.get("softcap"), slopes, max(c["lens"]))
-    again, _ = decode._decode(*args, None, True, grid=grid)
-    assert torch.equal(again, out), "keeping weights does not change the result, and a call repeats its bits"
+    # without weights the rows may be split otherwise (one launch, clusters); a call repeats its bits
+    out, lse = decode._decode(*args, None, True, grid=grid)
+    _check(out, lse, None, ora, dtype, c["D"], opt.get("softcap"), slopes, max(c["lens"]))
+    for keep in (None, w):
+        first, again = (decode._decode(*args, keep, True, grid=grid) for _ in range(2))
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
 @pytest.mark.gpu
