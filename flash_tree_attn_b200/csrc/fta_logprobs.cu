@@ -21,8 +21,10 @@
 // the warp's elements reach; the w-th largest of those bounds is reached by q w >= k elements.  Chunks
 // whose maximum reaches it (typically less than twice k; later, the k-th largest so far is the bound)
 // are listed, their elements shared out over the block and ranked by counting.  Looking at a chunk where
-// it was found would hold up its whole warp.  Where too many reach the bound (ties, masked vocabularies)
-// the exact one is found bit by bit instead.
+// it was found would hold up its whole warp.  Where more reach the bound than can be listed, the larger
+// elements are collected in one more pass and of the equal ones (ties, vocabularies masked with -inf or
+// the type's lowest value) the first in order, as many as are wanted; only where the larger ones alone
+// are too many is the exact bound found, bit by bit.
 #include <cooperative_groups.h>
 
 #include "fta_common.cuh"
@@ -31,14 +33,18 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 256;     // 4 blocks an SM: one computes while the others' chunks arrive
-constexpr int kWarps = kThreads / 32;
-constexpr int kChunks = 8;        // 16-byte chunks per thread
-constexpr int kListedChunks = 128;
-constexpr int kListed = 8 * kListedChunks;  // elements ranked by counting
-constexpr int kPending = 64;      // listed chunks that may wait for the next round
-constexpr int kMostRounds = 16;   // largest q; below 4 full warps a row has fewer than kListedChunks
+constexpr int kChunks = 8;        // 16-byte chunks per thread and round
 constexpr int kMostBlocks = 8;    // of a cluster, so of a row
+// 256 threads a row, 4 blocks an SM: one computes while the others' chunks arrive.  64 threads, 16 blocks an
+// SM, for many rows of a few thousand logits: such a block's time is its barriers and latencies.
+template <int THREADS> struct Cfg {
+  static constexpr int kWarps = THREADS / 32;
+  static constexpr int kBlocks = 1024 / THREADS;                   // per SM
+  static constexpr int kListedChunks = THREADS == 64 ? 128 : 256;
+  static constexpr int kListed = 8 * kListedChunks;                // elements ranked by counting
+  static constexpr int kPending = THREADS == 64 ? 0 : 64;          // listed chunks that may wait for the next round
+  static constexpr int kMostRounds = 32;                           // largest q: a warp's lanes
+};
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
@@ -127,14 +133,14 @@ __device__ __forceinline__ unsigned long long rank_key(uint32_t k, int token) {
 
 struct Sums { float m, s, t; };  // s and t (log2 units) relative to m
 
-template <int N> __device__ __forceinline__ int block_sum(int x, int* scratch) {
+template <int WARPS> __device__ __forceinline__ int block_sum(int x, int* scratch) {
   x = __reduce_add_sync(0xffffffffu, x);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
   __syncthreads();
   int sum = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum += scratch[i];
+  for (int i = 0; i < WARPS; ++i) sum += scratch[i];
   return sum;
 }
 
@@ -163,18 +169,19 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
 // grid = rows * (blocks of a cluster); block i of a row takes its rounds [i * rounds, (i + 1) * rounds) of
 // kThreads * kChunks chunks.  Chunks lie on 16-byte boundaries of memory, whatever the row's start; the few
 // elements before the first and behind the last are handed to one lane each.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobParams p, const int blocks, const int rounds) {
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kernel(const FtaLogprobParams p, const int blocks, const int rounds) {
   constexpr int VE = Vec<T>::n;
-  constexpr int kRound = kThreads * kChunks;
-  static_assert(kRound * VE <= 1 << 15, "the search over a round's tokens takes 16 steps");
-  __shared__ __align__(16) unsigned long long list[kListed + 2 * VE + FTA_MAX_TOP_K + 8];
+  constexpr int kRound = kThreads * kChunks, kWarps = Cfg<kThreads>::kWarps, kMostRounds = Cfg<kThreads>::kMostRounds;
+  constexpr int kListedChunks = Cfg<kThreads>::kListedChunks, kPending = Cfg<kThreads>::kPending;
+  // room for what waits from earlier rounds, a whole list, the row's edges, the likeliest so far, and zeros
+  __shared__ __align__(16) unsigned long long list[8 * kPending + Cfg<kThreads>::kListed + 2 * VE + FTA_MAX_TOP_K + 8];
   __shared__ unsigned long long best[FTA_MAX_TOP_K];  // the likeliest so far, in order; 0: none
   __shared__ Sums s_sums;
   __shared__ float s_a[kWarps], s_b[kWarps], s_c[kWarps];
   __shared__ int s_i[kWarps];
   __shared__ uint32_t s_key[kWarps];
-  __shared__ int s_n, s_listed;
+  __shared__ int s_n, s_larger, s_listed;
   __shared__ int s_where[kListedChunks];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long row = blockIdx.x / blocks;
@@ -184,8 +191,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
   const int start = min(head ? VE - head : 0, p.vocab);  // the first chunk's first element
   const int total = (p.vocab - start) / VE;               // chunks
   const int k = p.top_k;
-  if (tid < k) best[tid] = 0;
-  if (tid == 0) s_n = s_listed = 0;
+  for (int i = tid; i < k; i += kThreads) best[i] = 0;
+  if (tid == 0) s_n = s_larger = s_listed = 0;
   // the first block of a row answers for its tokens; their logits are asked for before all else
   auto logit_of = [&](int i, bool& inside) {
     const long long tok = p.tokens_are_i64 ? reinterpret_cast<const long long*>(p.tokens)[row * p.t_sr + i]
@@ -242,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     }
 
     if (round == 0 && k > 0) {
-      const int full = min(kWarps, chunks / 32);  // warps whose lanes all hold elements
+      // warps whose lanes all hold elements; one that holds part of them will do if k lanes have some
+      const int full = max(min(kWarps, chunks / 32), chunks >= k ? 1 : 0);
       const int q = full > 0 ? fta_cdiv(k, full) : kMostRounds + 1;
       uint32_t kth = 0;
       if (q <= kMostRounds && warp < full) {  // the warp's q-th largest lane maximum
@@ -301,12 +309,16 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     uint32_t reach = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) reach |= top[c] < bound ? 0u : 1u << c;
+    uint32_t larger_than = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) larger_than |= top[c] <= bound ? 0u : 1u << c;
     while (reach != 0) {
-      const int c = (__ffs(reach) - 1) * kThreads + tid;
+      const int bit = __ffs(reach) - 1, c = bit * kThreads + tid;
       reach &= reach - 1;
       if (c >= chunks) break;
       const int to = atomicAdd(&s_n, 1);
       if (to < kListedChunks) s_where[to] = base + c;
+      if ((larger_than >> bit) & 1) atomicAdd(&s_larger, 1);
     }
     if (edge >= 0 && !(edge_logit < bound)) list[atomicAdd(&s_listed, 1)] = rank_key(ordered(edge_logit), edge);
     __syncthreads();
@@ -325,27 +337,41 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     __syncthreads();
     if (over) {
       const int lo = start + base * VE, hi = lo + chunks * VE;
-      // The k-th largest value, bit by bit from the top: the largest key that at least k elements reach.
-      uint32_t key = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t at_least = key | (1u << bit);
-        int count = 0;
-        for (int i = lo + tid; i < hi; i += kThreads) count += ordered(to_float(x[i])) >= at_least;
-        if (block_sum<kWarps>(count, s_i) >= k) key = at_least;
-      }
-      // Of the elements equal to it the lowest tokens are wanted: those below the least `end` that makes k.
-      int end = lo;
-      for (int step = 1 << 15; step > 0; step >>= 1) {  // a round holds at most 2^15 elements
-        int count = 0;
-        for (int i = lo + tid; i < hi; i += kThreads) {
-          const uint32_t o = ordered(to_float(x[i]));
-          count += o > key || (o == key && i < end + step);
+      uint32_t key = ordered(bound);
+      if (s_larger > kListedChunks) {
+        // the k-th largest value, bit by bit from the top: the largest key that at least k elements reach
+        key = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+          const uint32_t at_least = key | (1u << bit);
+          int count = 0;
+          for (int i = lo + tid; i < hi; i += kThreads) count += ordered(to_float(x[i])) >= at_least;
+          if (block_sum<kWarps>(count, s_i) >= k) key = at_least;
         }
-        if (block_sum<kWarps>(count, s_i) < k) end += step;
       }
+      int larger = 0;
       for (int i = lo + tid; i < hi; i += kThreads) {
         const uint32_t o = ordered(to_float(x[i]));
-        if (o > key || (o == key && i <= end)) list[atomicAdd(&s_listed, 1)] = rank_key(o, i);
+        if (o > key) {
+          list[atomicAdd(&s_listed, 1)] = rank_key(o, i);
+          ++larger;
+        }
+      }
+      int wanted = k - block_sum<kWarps>(larger, s_i);
+      for (int first = lo; first < hi && wanted > 0; first += kThreads) {  // in order, until there are enough
+        const int i = first + tid;
+        const uint32_t o = i < hi ? ordered(to_float(x[i])) : 0u;  // 0: below every key
+        const unsigned who = __ballot_sync(0xffffffffu, o == key && i < hi);
+        if (lane == 0) s_key[warp] = __popc(who);
+        __syncthreads();
+        int before = __popc(who & ((1u << lane) - 1)), all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          before += w < warp ? (int)s_key[w] : 0;
+          all += s_key[w];
+        }
+        if (o == key && i < hi && before < wanted) list[atomicAdd(&s_listed, 1)] = rank_key(o, i);
+        wanted -= all;
+        __syncthreads();
       }
       __syncthreads();
     }
@@ -356,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     }
     if (tid < 8) list[n + tid] = 0;
     __syncthreads();
-    if (tid == 0) s_n = s_listed = 0;
+    if (tid == 0) s_n = s_larger = s_listed = 0;
     for (int i = tid; i < n; i += kThreads) {
       const unsigned long long own = list[i];
       const int before = larger(list, n, own);
@@ -407,8 +433,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     if (block != 0) return;
   } else {
     __syncthreads();
-    for (int i = tid; i < k; i += kThreads) list[i] = best[i];
-    if (tid < 8) list[k + tid] = 0;
+    for (int i = tid; i < k + 8; i += kThreads) list[i] = i < k ? best[i] : 0;
     __syncthreads();
   }
   m = sums.m;
@@ -426,11 +451,22 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
     const float v = i == tid ? asked : logit_of(i, inside);
     p.logprobs[row * p.n_tokens + i] = inside ? log_p(v) : -INFINITY;
   }
-  const int n = blocks * k;
-  for (int i = tid; i < n; i += kThreads) {
+  // Few keys are counted; of many, a key's rank is its place in its own block's list, which is in order, and
+  // what a binary search finds before it in the others.
+  const bool few = blocks * k <= 64;
+  for (int i = tid; i < blocks * k; i += kThreads) {
     const unsigned long long own = list[i];
     if (own == 0) continue;
-    const int before = larger(list, n, own);
+    int before = few ? larger(list, blocks * k, own) : i % k;
+    for (int other = 0; other < blocks && !few; ++other) {
+      if (other == i / k) continue;
+      int lo = 0, hi = k;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (list[other * k + mid] > own) lo = mid + 1; else hi = mid;
+      }
+      before += lo;
+    }
     if (before < k) {
       p.top_logprobs[row * k + before] = log_p(unordered((uint32_t)(own >> 32)));
       p.top_ids[row * k + before] = (int64_t)(0xffffffffu - (uint32_t)own);
@@ -438,17 +474,12 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const FtaLogprobPa
   }
 }
 
-int pieces_of(const FtaLogprobParams& p) {
-  const int ve = p.dtype == FTA_DTYPE_F32 ? 4 : 8;
-  return p.vocab < ve ? 1 : fta_cdiv(p.vocab / ve, kThreads * kChunks);
-}
-
-template <typename T>
-int run(const FtaLogprobParams& p, cudaStream_t st) {
-  const int pieces = pieces_of(p);
+template <typename T, int THREADS>
+int run_with(const FtaLogprobParams& p, cudaStream_t st) {
+  const int chunks = p.vocab / Vec<T>::n, pieces = chunks > 0 ? fta_cdiv(chunks, THREADS * kChunks) : 1;
   // Blocks per row: enough to fill the machine, and no more.  A wave of blocks lasts as long as its
   // rounds, and about one round more for the start and the end of a block, another one for a cluster's join.
-  const int slots = 148 * 4;
+  const int slots = 148 * Cfg<THREADS>::kBlocks;
   int blocks = 1, rounds = pieces;
   long long least = 0x7fffffffffffffffLL;
   for (int n = 1; n <= kMostBlocks && n <= pieces; ++n) {
@@ -461,10 +492,16 @@ int run(const FtaLogprobParams& p, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows * blocks); cfg.blockDim = dim3(kThreads); cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprob_kernel<T>, p, blocks, rounds);
+  cfg.gridDim = dim3(p.rows * blocks); cfg.blockDim = dim3(THREADS); cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = blocks > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprob_kernel<T, THREADS>, p, blocks, rounds);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
+}
+
+template <typename T>
+int run(const FtaLogprobParams& p, cudaStream_t st) {
+  const bool small = p.vocab / Vec<T>::n <= 64 * kChunks && p.rows > 148 * 4;
+  return small ? run_with<T, 64>(p, st) : run_with<T, 256>(p, st);
 }
 
 }  // namespace

@@ -43,7 +43,8 @@ def _tokens(rows, V, n, g, dtype=torch.int64):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,V,k", [(1, 1, 1), (3, 2, 2), (2, 7, 3), (5, 64, 64), (3, 100, 64), (2, 255, 5), (2, 2049, 20), (3, 4097, 64), (2, 16384, 1),
-                                      (2, 32768, 33), (2, 32769, 64), (300, 1000, 8), (3, 50257, 20), (2, 128256, 5), (1, 262144, 64), (2, 300001, 10), (4, 5000, 0)])
+                                      (2, 32768, 33), (2, 32769, 64), (300, 1000, 8), (3, 50257, 20), (2, 128256, 5), (1, 262144, 64), (2, 300001, 10), (4, 5000, 0),
+                                      (700, 1000, 64), (601, 4095, 20), (601, 33, 5), (2, 16500, 64), (20, 56697, 64)])
 def test_matches_the_formula(dtype, rows, V, k):
     import flash_tree_attn_b200 as fta
 
@@ -69,20 +70,20 @@ def test_rows_that_start_anywhere(dtype, shift):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["equal", "two values", "masked", "all masked", "nan", "inf", "rising", "one high", "far", "lowest", "lowest and masked"])
-@pytest.mark.parametrize("V", [50, 3000, 70001])
-def test_rows_that_tie_or_are_masked(kind, V):
+@pytest.mark.parametrize("kind", ["equal", "two values", "masked", "all masked", "nan", "inf", "rising", "one high", "far", "lowest", "lowest and masked", "blocks"])
+@pytest.mark.parametrize("V,rows", [(50, 4), (3000, 4), (70001, 4), (2999, 601)])
+def test_rows_that_tie_or_are_masked(kind, V, rows):
     import flash_tree_attn_b200 as fta
 
     g = torch.Generator().manual_seed(V)
-    x = torch.randn(4, V, generator=g)
+    x = torch.randn(rows, V, generator=g)
     if kind == "equal":
         x[:] = 1.5
     elif kind == "two values":
         x = (x > 1.0).float()
         x[0, ::2] = -0.0
     elif kind == "masked":
-        keep = torch.rand(4, V, generator=g) < 4.0 / V
+        keep = torch.rand(rows, V, generator=g) < 4.0 / V
         x = x.masked_fill(~keep, float("-inf"))
         x[:, V // 2] = 0.0
     elif kind == "all masked":
@@ -94,14 +95,17 @@ def test_rows_that_tie_or_are_masked(kind, V):
     elif kind == "inf":
         x[1, 7] = float("inf")
     elif kind == "rising":
-        x = torch.arange(V).float().expand(4, V) * 1e-3
+        x = torch.arange(V).float().expand(rows, V) * 1e-3
     elif kind == "one high":
         x[:, 3] = 300.0
+    elif kind == "blocks":  # what is large sits together, in different places of each row
+        for r in range(rows):
+            x[r, (r * 977) % V: (r * 977) % V + 2500] += 50.0
     elif kind == "far":
         x = x - 20000.0
     for dtype in (torch.float32, torch.bfloat16, torch.float16):
         if kind.startswith("lowest"):  # masked with the type's lowest value, and two rows of nothing else
-            x = torch.randn(4, V, generator=g)
+            x = torch.randn(rows, V, generator=g)
             x[:2] = torch.finfo(dtype).min
             x[2, 1:] = torch.finfo(dtype).min
             if kind.endswith("masked"):
@@ -109,7 +113,7 @@ def test_rows_that_tie_or_are_masked(kind, V):
         if dtype == torch.float16 and kind == "far":
             x = x / 4
         y = x.to(dtype).cuda()
-        t = _tokens(4, V, 2, g)
+        t = _tokens(rows, V, 2, g)
         _check(y, t, 40, fta.token_logprobs(y, t, 40))
 
 
