@@ -5,14 +5,18 @@
 // writes the list of kept rows and their weights in order.  Digits are 11, 11 and 10 bits wide: the top
 // 11 are the exponent and two bits more, over which weights spread; with 8 bits most of a warp's
 // counts met in the same few bins, one after the other.
-// Move: new row i takes old row kept[i] >= i.  A block owns a column slice of one head's K or V and
-// walks the list in chunks: all of a chunk's rows are read, then written.  A write goes to rows below
+// Move: new row i takes old row kept[i] >= i.  A block, or a cluster of them, owns a column slice of one
+// head's K or V and walks the list in chunks: all of a chunk's rows are read, then written.  A write goes to rows below
 // the chunk's end, a later chunk's rows lie at or above it, so reads never see a write, and the next
 // chunk's reads are under way while this one's rows are written.
 //
 // What bounds it: the kept rows of K and V are read and written once (8 D bytes a row); the weights
 // are small against that.
+#include <cooperative_groups.h>
+
 #include "fta_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -22,22 +26,22 @@ constexpr int kMove = 256;
 constexpr int kAhead = 3;         // rows per thread and chunk
 constexpr int kBins = 2048;
 
-// order of floats as unsigned integers; -0 and +0 alike, NaN on top
-__device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
+// Weights are handled as their bits throughout: arithmetic would take the smallest ones for zeros.
+// Their order as unsigned integers; -0 and +0 alike, NaN on top.
+__device__ __forceinline__ uint32_t ordered(uint32_t b) {
   if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
   if (b == 0x80000000u) return b;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
 // Moves w[from, from + n) to w[to, to + n), to <= from: a chunk is read, then written.
-template <typename F> __device__ __forceinline__ void move_up(float* w, int to, int n, F&& from) {
+template <typename F> __device__ __forceinline__ void move_up(uint32_t* w, int to, int n, F&& from) {
   for (int base = 0; base < n; base += 4 * kSelect) {
-    float x[4];
+    uint32_t x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = base + u * kSelect + (int)threadIdx.x;
-      x[u] = i < n ? w[from(i)] : 0.f;
+      x[u] = i < n ? w[from(i)] : 0u;
     }
     __syncthreads();
 #pragma unroll
@@ -50,7 +54,7 @@ template <typename F> __device__ __forceinline__ void move_up(float* w, int to, 
 
 // `room`: weights that the dynamic shared memory holds; a longer sequence's are read again in every pass
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictParams p, const int room) {
-  extern __shared__ float s_w[];
+  extern __shared__ __align__(16) uint32_t s_w[];
   __shared__ int hist[kBins];
   __shared__ int s_bin, s_left;
   __shared__ int s_equal[32], s_larger[32];
@@ -63,14 +67,31 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictPar
     for (int i = tid; i < p.budget; i += kSelect) kept[i] = i < L ? i : -1;
     return;
   }
-  float* w = p.row_weights + b * p.rw_sb + h * p.rw_sh;
+  uint32_t* w = reinterpret_cast<uint32_t*>(p.row_weights) + b * p.rw_sb + h * p.rw_sh;
   const int n = L - p.recent, want = p.budget - p.recent;  // n > want
 
   if (want > 0) {
     const bool held = n <= room;
-    if (held)
+    if (held) {
+#pragma unroll 8
       for (int r = tid; r < n; r += kSelect) s_w[r] = w[r];
-    auto key = [&](int r) { return ordered(held ? s_w[r] : w[r]); };
+    }
+    // the keys of rows r .. r + 3, r a multiple of 4; 0, which is below every weight, past the end
+    auto keys = [&](int r, uint32_t (&k)[4]) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (held) {
+        if (r < n) x = *reinterpret_cast<const uint4*>(s_w + r);  // n <= room, a multiple of 4
+      } else {
+        if (r < n) x.x = w[r];
+        if (r + 1 < n) x.y = w[r + 1];
+        if (r + 2 < n) x.z = w[r + 2];
+        if (r + 3 < n) x.w = w[r + 3];
+      }
+      k[0] = r < n ? ordered(x.x) : 0u;
+      k[1] = r + 1 < n ? ordered(x.y) : 0u;
+      k[2] = r + 2 < n ? ordered(x.z) : 0u;
+      k[3] = r + 3 < n ? ordered(x.w) : 0u;
+    };
 
     // the want-th largest of w[0, n): its bits from the top, `left` counts down to its rank among equals
     uint32_t prefix = 0, mask = 0;
@@ -81,9 +102,12 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictPar
       hist[tid] = 0;
       hist[tid + kSelect] = 0;
       __syncthreads();
-      for (int r = tid; r < n; r += kSelect) {
-        const uint32_t k = key(r);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit], 1);
+      for (int r = 4 * tid; r < n; r += 4 * kSelect) {
+        uint32_t k[4];
+        keys(r, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((k[e] & mask) == prefix && k[e] != 0u) atomicAdd(&hist[(k[e] >> shift) & digit], 1);
       }
       __syncthreads();
       // a thread holds bins 2047 - 2 tid and the one below; `above` counts the bins that come before
@@ -110,30 +134,48 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictPar
 
     // Larger ones are kept, and the first `left` equal ones.  Each warp counts both in a stretch of rows,
     // then, knowing what lies before it, writes its part of the list.
-    const int per = fta_cdiv(fta_cdiv(n, 32), 32) * 32, r0 = min(n, warp * per), r1 = min(n, r0 + per);
+    const int per = fta_cdiv(fta_cdiv(n, 32), 128) * 128, r0 = warp * per, r1 = min(n, r0 + per);
     int equal = 0, larger = 0;
-    for (int r = r0 + lane; r - lane < r1; r += 32) {
-      const uint32_t k = r < r1 ? key(r) : 0u;  // 0: below every weight
-      equal += __popc(__ballot_sync(0xffffffffu, k == prefix));
-      larger += __popc(__ballot_sync(0xffffffffu, k > prefix));
+    for (int r = r0 + 4 * lane; r < r1; r += 128) {
+      uint32_t k[4];
+      keys(r, k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { equal += k[e] == prefix; larger += k[e] > prefix; }
     }
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    larger = __reduce_add_sync(0xffffffffu, larger);
     __syncthreads();  // s_equal of the last pass has been read
     if (lane == 0) { s_equal[warp] = equal; s_larger[warp] = larger; }
     __syncthreads();
     equal = __reduce_add_sync(0xffffffffu, lane < warp ? s_equal[lane] : 0);
     larger = __reduce_add_sync(0xffffffffu, lane < warp ? s_larger[lane] : 0);
-    for (int r = r0 + lane; r - lane < r1; r += 32) {
-      const uint32_t k = r < r1 ? key(r) : 0u;
-      const unsigned eqs = __ballot_sync(0xffffffffu, k == prefix), gts = __ballot_sync(0xffffffffu, k > prefix);
-      const unsigned below = (1u << lane) - 1;
-      const int e = equal + __popc(eqs & below);  // equal ones before this row
-      if (k > prefix || (k == prefix && e < left)) {
-        const int at = larger + __popc(gts & below) + min(e, left);
-        kept[at] = r;
-        if (held) w[at] = s_w[r];  // nobody reads w[0, n) any more
+    for (int first = r0; first < r1; first += 128) {
+      const int r = first + 4 * lane;
+      uint32_t k[4];
+      keys(r, k);
+      int both = 0;  // equal ones in the low half, larger ones in the high half
+#pragma unroll
+      for (int e = 0; e < 4; ++e) both += (k[e] == prefix ? 1 : 0) + (k[e] > prefix ? 1 << 16 : 0);
+      int sum = both;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += t;
       }
-      equal += __popc(eqs);
-      larger += __popc(gts);
+      int e_before = equal + ((sum - both) & 0xffff), g_before = larger + ((sum - both) >> 16);
+      const int all = __shfl_sync(0xffffffffu, sum, 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (k[e] > prefix || (k[e] == prefix && e_before < left)) {
+          const int at = g_before + min(e_before, left);
+          kept[at] = r + e;
+          if (held) w[at] = s_w[r + e];  // nobody reads w[0, n) any more
+        }
+        e_before += k[e] == prefix;
+        g_before += k[e] > prefix;
+      }
+      equal += all & 0xffff;
+      larger += all >> 16;
     }
     __syncthreads();
     if (!held) move_up(w, 0, want, [&](int i) { return kept[i]; });
@@ -141,15 +183,16 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictPar
   for (int i = tid; i < p.recent; i += kSelect) kept[want + i] = n + i;
   move_up(w, want, p.recent, [&](int i) { return n + i; });
   __syncthreads();
-  for (int r = p.budget + tid; r < L; r += kSelect) w[r] = 0.f;
+  for (int r = p.budget + tid; r < L; r += kSelect) w[r] = 0u;
 }
 
-// grid = (B * Hkv, K or V, column slices); a row of a slice is `chunks` 16-byte chunks
-__global__ void __launch_bounds__(kMove, 4) evict_move_kernel(const FtaEvictParams p, const int chunks) {
-  const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
-  const int* kept = p.kept + (long long)blockIdx.x * p.budget;
+// grid = (B * Hkv * blocks of a cluster, K or V, column slices); a row of a slice is `chunks` 16-byte chunks
+__global__ void __launch_bounds__(kMove, 4) evict_move_kernel(const FtaEvictParams p, const int chunks, const int blocks) {
+  const int unit = blockIdx.x / blocks, rank = blockIdx.x - unit * blocks;
+  const int b = unit / p.Hkv, h = unit - b * p.Hkv;
+  const int* kept = p.kept + (long long)unit * p.budget;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (blockIdx.y == 0 && blockIdx.z == 0 && h == 0 && threadIdx.x == 0) {
+  if (rank == 0 && blockIdx.y == 0 && blockIdx.z == 0 && h == 0 && threadIdx.x == 0) {
     // the select kernel has read the lengths, and this one does not
     const int L = min(fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx), p.budget);
     if (p.len_is_i64) reinterpret_cast<long long*>(p.kv_seq_len)[b] = L;
@@ -167,7 +210,7 @@ __global__ void __launch_bounds__(kMove, 4) evict_move_kernel(const FtaEvictPara
     lo = from;
   }
   const long long sb = blockIdx.y ? p.v_sb : p.k_sb, sh = blockIdx.y ? p.v_sh : p.k_sh, st = blockIdx.y ? p.v_st : p.k_st;
-  const int per = kMove / chunks, mine = threadIdx.x / chunks, c = threadIdx.x - mine * chunks;
+  const int per = kMove / chunks * blocks, mine = kMove / chunks * rank + threadIdx.x / chunks, c = threadIdx.x % chunks;
   uint16_t* cache = (uint16_t*)(blockIdx.y ? p.v_cache : p.k_cache) + h * sh + ((long long)blockIdx.z * chunks + c) * 8;
   const int page_bits = (p.page_size & (p.page_size - 1)) == 0 ? __ffs(p.page_size) - 1 : -1;  // a division costs as much as a row's copy
   const int* table = p.block_table + b * p.bt_sb;
@@ -209,7 +252,8 @@ __global__ void __launch_bounds__(kMove, 4) evict_move_kernel(const FtaEvictPara
   for (int base = lo; base < p.budget; base += chunk) {
     has_next = read(next);
     ask(base + 2 * chunk);
-    __syncthreads();  // everybody has read this chunk
+    if (blocks == 1) __syncthreads();  // everybody has read this chunk
+    else cg::this_cluster().sync();
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       uint4* dst = (has_now >> u) & 1 ? row_at(base + u * per + mine) : nullptr;
@@ -243,19 +287,22 @@ extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
     if (e != cudaSuccess) return fta_cuda_fail(e);
     configured |= 1ull << (dev & 63);
   }
-  const int room = p->ctx < kKeys ? p->ctx : kKeys;
+  const int room = p->ctx < kKeys ? (p->ctx + 3) / 4 * 4 : kKeys;
   evict_select_kernel<<<p->B * p->Hkv, kSelect, room * 4, st>>>(*p, room);
-  // column slices until there are blocks for every SM; no slice below a 32-byte sector
-  int slices = 1;
-  while ((long long)p->B * p->Hkv * 2 * slices < 2 * 148 && p->D / 8 / slices > 2) slices *= 2;
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return fta_cuda_fail(e);
-  cudaLaunchAttribute attr[1];
+  // Blocks until every SM has about two: first the blocks of a cluster, which share out a chunk's rows, then
+  // column slices, none below a 32-byte sector.  A block moves some 20 GB/s: one unit of 13580 rows of 128 in
+  // 16 blocks (slices of 32 bytes alone) took 25 us, in 32 (clusters of 8, 128 bytes) 15, in 128 (both) 6.
+  int blocks = 1, slices = 1;
+  while ((long long)p->B * p->Hkv * 2 * blocks < 2 * 148 && blocks < 8) blocks *= 2;
+  while ((long long)p->B * p->Hkv * 2 * blocks * slices < 2 * 148 && p->D / 8 / slices > 2) slices *= 2;
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p->B * p->Hkv, 2, slices); cfg.blockDim = dim3(kMove); cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, *p, p->D / 8 / slices);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(p->B * p->Hkv * blocks, 2, slices); cfg.blockDim = dim3(kMove); cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = blocks > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, *p, p->D / 8 / slices, blocks);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
