@@ -289,12 +289,16 @@ extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
   }
   const int room = p->ctx < kKeys ? (p->ctx + 3) / 4 * 4 : kKeys;
   evict_select_kernel<<<p->B * p->Hkv, kSelect, room * 4, st>>>(*p, room);
-  // Blocks until every SM has about two: first the blocks of a cluster, which share out a chunk's rows, then
-  // column slices, none below a 32-byte sector.  A block moves some 20 GB/s: one unit of 13580 rows of 128 in
-  // 16 blocks (slices of 32 bytes alone) took 25 us, in 32 (clusters of 8, 128 bytes) 15, in 128 (both) 6.
+  // Blocks until every SM has three (not every unit has rows to move): first the blocks of a cluster, which
+  // share out a chunk's rows, then column slices down to 64 bytes, and to a 32-byte sector only where there
+  // are fewer than two a SM.  A block moves some 20 GB/s: one unit of 13580 rows of 128 in 16 blocks (slices
+  // of 32 bytes alone) took 25 us, in 32 (clusters of 8, 128 bytes) 15, in 128 (both) 6.
+  const long long units = (long long)p->B * p->Hkv * 2;
+  const int width = p->D / 8;
   int blocks = 1, slices = 1;
-  while ((long long)p->B * p->Hkv * 2 * blocks < 2 * 148 && blocks < 8) blocks *= 2;
-  while ((long long)p->B * p->Hkv * 2 * blocks * slices < 2 * 148 && p->D / 8 / slices > 2) slices *= 2;
+  while (units * blocks < 3 * 148 && blocks < 8) blocks *= 2;
+  while (units * blocks * slices < 4 * 148 && blocks == 8 && width / slices > 4) slices *= 2;
+  while (units * blocks * slices < 2 * 148 && width / slices > 2) slices *= 2;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
