@@ -215,6 +215,30 @@ __host__ __device__ __forceinline__ bool fta_row(const FtaParams& p, const FtaGe
 int fta_cuda_fail(cudaError_t e);
 
 #ifdef __CUDACC__
+// Programmatic stream serialization (the kernels beside stage 1 and 2): a kernel launched by
+// fta_launch_after is set up while the kernel before it in the stream drains.  Its blocks begin with
+// fta_after_previous: what follows is set up early in turn, and nothing is read or written before the
+// kernel before this one has finished.  Every block does so, the idle ones too, so that a finished kernel
+// means that all before it have finished.
+__device__ __forceinline__ void fta_after_previous() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// cluster: blocks of a thread-block cluster (grid.x a multiple of it), 1 for none
+template <typename... Params, typename... Args>
+cudaError_t fta_launch_after(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- device helpers ----------------------------------------------------------------------
 
 // BALANCED workspace: partial O rows [2*grid][R][D] fp32, partial LSEs [2*grid][R] fp32, then one

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const FtaEvictPar
   __shared__ int s_equal[32], s_larger[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the move's blocks wait for this grid's end
+  fta_after_previous();
   const int L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx);
   int* kept = p.kept + (long long)blockIdx.x * p.budget;
   if (L <= p.budget) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kMove, 4) evict_move_kernel(const FtaEvictPara
   const int unit = blockIdx.x / blocks, rank = blockIdx.x - unit * blocks;
   const int b = unit / p.Hkv, h = unit - b * p.Hkv;
   const int* kept = p.kept + (long long)unit * p.budget;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  fta_after_previous();
   if (rank == 0 && blockIdx.y == 0 && blockIdx.z == 0 && h == 0 && threadIdx.x == 0) {
     // the select kernel has read the lengths, and this one does not
     const int L = min(fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx), p.budget);
@@ -288,7 +288,8 @@ extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
     configured |= 1ull << (dev & 63);
   }
   const int room = p->ctx < kKeys ? (p->ctx + 3) / 4 * 4 : kKeys;
-  evict_select_kernel<<<p->B * p->Hkv, kSelect, room * 4, st>>>(*p, room);
+  e = fta_launch_after(evict_select_kernel, dim3(p->B * p->Hkv), kSelect, room * 4, st, 1, *p, room);
+  if (e != cudaSuccess) return fta_cuda_fail(e);
   // Blocks until every SM has three (not every unit has rows to move): first the blocks of a cluster, which
   // share out a chunk's rows, then column slices down to 64 bytes, and to a 32-byte sector only where there
   // are fewer than two a SM.  A block moves some 20 GB/s: one unit of 13580 rows of 128 in 16 blocks (slices
@@ -299,14 +300,6 @@ extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
   while (units * blocks < 3 * 148 && blocks < 8) blocks *= 2;
   while (units * blocks * slices < 4 * 148 && blocks == 8 && width / slices > 4) slices *= 2;
   while (units * blocks * slices < 2 * 148 && width / slices > 2) slices *= 2;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(p->B * p->Hkv * blocks, 2, slices); cfg.blockDim = dim3(kMove); cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = blocks > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, *p, p->D / 8 / slices, blocks);
+  e = fta_launch_after(evict_move_kernel, dim3(p->B * p->Hkv * blocks, 2, slices), kMove, 0, st, blocks, *p, width / slices, blocks);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }

@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
   const int start = min(head ? VE - head : 0, p.vocab);  // the first chunk's first element
   const int total = (p.vocab - start) / VE;               // chunks
   const int k = p.top_k;
+  fta_after_previous();
   for (int i = tid; i < k; i += kThreads) best[i] = 0;
   if (tid == 0) s_n = s_larger = s_listed = 0;
   // the first block of a row answers for its tokens; their logits are asked for before all else
@@ -488,13 +489,7 @@ int run_with(const FtaLogprobParams& p, cudaStream_t st) {
     const long long cost = (((long long)p.rows * n + slots - 1) / slots) * (r + (n > 1 ? 2 : 1));
     if (cost < least) { least = cost; blocks = n; rounds = r; }
   }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows * blocks); cfg.blockDim = dim3(THREADS); cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = blocks > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprob_kernel<T, THREADS>, p, blocks, rounds);
+  const cudaError_t e = fta_launch_after(logprob_kernel<T, THREADS>, dim3(p.rows * blocks), THREADS, 0, st, blocks, p, blocks, rounds);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
 

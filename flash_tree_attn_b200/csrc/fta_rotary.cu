@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const FtaRotaryPara
   __shared__ float2 cs[TOK][128];
   __shared__ long long s_dst[2][TOK];  // where the tokens' cache rows start (K, V); -1: nowhere
   const int b = blockIdx.y, i0 = blockIdx.x * TOK;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // only the lengths' growth is launched to wait
+  fta_after_previous();
 
   const int rot16 = p.n_freq / 8;  // lane tasks of a row that turn (half); 1 << row_bits tasks in all
   const int heads = p.H + p.Hkv + (APPEND ? p.Hkv : 0);
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const FtaRotaryPara
 
 __global__ void grow_lengths_kernel(const FtaRotaryParams p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // every block of the append has read the lengths
+  fta_after_previous();  // every block of the append has read the lengths
   if (b >= p.B) return;
   const long long L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx) + (long long)p.Q;
   const int to = (int)(L < p.ctx ? L : p.ctx);
@@ -204,20 +204,12 @@ int launch(const FtaRotaryParams* p, cudaStream_t st) {
   const dim3 grid(four ? (p->Q + 3) / 4 : p->Q, p->B);
   const int bits = p->D == 32 ? 1 : p->D == 64 ? 2 : p->D == 128 ? 3 : 4;
   const bool f16 = p->dtype == FTA_DTYPE_F16;
-  if (four && f16) rotary_kernel<__half, APPEND, 4><<<grid, kThreads, 0, st>>>(*p, bits);
-  else if (four) rotary_kernel<__nv_bfloat16, APPEND, 4><<<grid, kThreads, 0, st>>>(*p, bits);
-  else if (f16) rotary_kernel<__half, APPEND, 1><<<grid, kThreads, 0, st>>>(*p, bits);
-  else rotary_kernel<__nv_bfloat16, APPEND, 1><<<grid, kThreads, 0, st>>>(*p, bits);
-  cudaError_t e = cudaGetLastError();
-  if (APPEND && grid.x > 1 && e == cudaSuccess) {
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((p->B + 127) / 128); cfg.blockDim = dim3(128); cfg.stream = st;
-    cfg.attrs = attr; cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, grow_lengths_kernel, *p);
-  }
+  cudaError_t e;
+  if (four && f16) e = fta_launch_after(rotary_kernel<__half, APPEND, 4>, grid, kThreads, 0, st, 1, *p, bits);
+  else if (four) e = fta_launch_after(rotary_kernel<__nv_bfloat16, APPEND, 4>, grid, kThreads, 0, st, 1, *p, bits);
+  else if (f16) e = fta_launch_after(rotary_kernel<__half, APPEND, 1>, grid, kThreads, 0, st, 1, *p, bits);
+  else e = fta_launch_after(rotary_kernel<__nv_bfloat16, APPEND, 1>, grid, kThreads, 0, st, 1, *p, bits);
+  if (APPEND && grid.x > 1 && e == cudaSuccess) e = fta_launch_after(grow_lengths_kernel, dim3((p->B + 127) / 128), 128, 0, st, 1, *p);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
 

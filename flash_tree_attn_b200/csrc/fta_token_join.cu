@@ -26,8 +26,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenP
   const int2* desc = reinterpret_cast<const int2*>(wsb + ws.desc);
   const float* lse2 = reinterpret_cast<const float*>(wsb + ws.lse2);
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  fta_after_previous();
 
   const int L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx);
   const int row0 = blockIdx.y * chunk_rows;
@@ -237,13 +236,7 @@ extern "C" int fta_decode_token(const FtaTokenParams* p, void* stream) {
   if (e != cudaSuccess) return fta_cuda_fail(e);
   if (g.family == 1) return FTA_OK;
   const int chunk = 4 * kThreads;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p->B * p->Hkv, weights ? (p->ctx + chunk - 1) / chunk + (p->ctx == 0) : 1);
-  cfg.blockDim = dim3(kThreads); cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, token_join_kernel, *p, g, chunk);
+  const dim3 grid(p->B * p->Hkv, weights ? (p->ctx + chunk - 1) / chunk + (p->ctx == 0) : 1);
+  e = fta_launch_after(token_join_kernel, grid, kThreads, 0, st, 1, *p, g, chunk);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }

@@ -111,8 +111,8 @@ def _decode(q, k, v, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv
         slopes = alibi_slopes.data_ptr()
     weights = row_weights is not None
     rw, rw_sb, rw_sh = check_weights(row_weights, B, Hkv, ctx, dev) if weights else (0, 0, 0)
-    out = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, H, 1, D), dtype=dt, device=q.device)
-    lse = torch.empty((B, H, 1), dtype=_f32, device=q.device) if return_lse else None
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(B, H, 1, D, dtype=dt, device=q.device)
+    lse = torch.empty(B, H, 1, dtype=_f32, device=q.device) if return_lse else None
     if B and H:
         size = _workspace(lib, dev, B, H, Hkv, D, ctx, code, weights, window or 0, grid)
         ws = out.new_empty(size) if size else None  # `size` elements of two bytes each
@@ -223,7 +223,7 @@ def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: i
     rw, rw_sb, rw_sh = check_weights(row_weights, B, Hkv, ctx, dev)
     budget, recent = int(budget), int(recent)
     assert 1 <= budget <= 0x7fffffff and 0 <= recent <= budget, "1 <= budget and 0 <= recent <= budget"
-    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_cache.device)
+    kept = torch.empty(B, Hkv, budget, dtype=torch.int32, device=k_cache.device)
     if B and Hkv:
         launch(lib.fta_evict_rows, pack_evict(*kr, *vr, kv_seq_len.data_ptr(), table, table_sb, rw, rw_sb, rw_sh, kept.data_ptr(),
                                               is64, B, Hkv, D, ctx, page, n_pages, budget, recent, 0), dev, "fta_evict_rows")

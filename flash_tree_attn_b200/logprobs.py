@@ -55,7 +55,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if one != 1 and V > 1:
         logits = logits.contiguous()
         row_stride = V
-    entropy = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    # sizes one by one: a tuple of them costs half as much again to read
+    entropy = torch.empty(*lead, dtype=torch.float32, device=logits.device) if lead else logits.new_empty((), dtype=torch.float32)
     lse = torch.empty_like(entropy)
     n = tp = token_stride = t64 = 0
     lp = top_lp = top_ids = None
@@ -65,7 +66,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         assert t64 is not None and tokens.get_device() == dev and len(ts) == len(shape) and ts[:-1] == lead, \
             "tokens must be [.., n] int32 or int64 on the logits' device, with the logits' leading sizes"
         n = ts[-1]
-        lp = entropy.new_empty(ts)
+        lp = entropy.new_empty(*ts)
         if len(ts) != 2:
             tokens = tokens.reshape(rows, n)
         token_stride, one = tokens.stride()
@@ -74,9 +75,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
             token_stride = n
         tp = tokens.data_ptr()
     if top_k:
-        top = (*lead, top_k)
-        top_lp = entropy.new_empty(top)
-        top_ids = tokens.new_empty(top) if t64 else torch.empty(top, dtype=torch.int64, device=logits.device)
+        top_lp = entropy.new_empty(*lead, top_k)
+        top_ids = torch.empty_like(top_lp, dtype=torch.int64)
     if rows:
         launch(lib.fta_token_logprobs, pack_logprob(
             logits.data_ptr(), row_stride, tp, token_stride, lp.data_ptr() if n else 0, entropy.data_ptr(), lse.data_ptr(),
