@@ -36,7 +36,8 @@ __global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenP
     const int gt = hh / g.R, r = hh - gt * g.R, h = kvh * G + hh;
     const int j = kvh * g.n_gt + gt;
     float total = -INFINITY;
-    const int2 d = L > 0 ? desc[(long long)b * g.U + j] : make_int2(0, 0);
+    int2 d = desc[(long long)b * g.U + j];  // asked for together with the length, which says whether it was written
+    if (L == 0) d = make_int2(0, 0);
     if (d.x == 1) {  // stage 1 wrote the rows itself
       if (weights) total = lse2[(long long)b * p.H + h];
     } else if (d.x > 1) {
@@ -171,7 +172,7 @@ int geometry(const FtaTokenParams& p, FtaGeom& g) {
   g.n_tree = 0;
   g.min_per = 1;
   g.fixed_max_splits = 0; g.family = 0; g.cs = 1;
-  g.pad = 1;
+  g.pad = 4;  // as the warp-MMA family; 0 to 4 lie within 2 % of each other
   g.grid = p.grid_override;
   if (p.grid_override == 0) {
     int dev = 0;
