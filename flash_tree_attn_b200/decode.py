@@ -20,6 +20,7 @@ from ._lib import launch, pack_evict, pack_token, rows_of
 _DT = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _LEN = {torch.int32: 0, torch.int64: 1}  # -> is int64
 _HEAD_DIMS = (32, 64, 128, 256)
+_MOST_ROWS = 0x7fffff00  # of a sequence: row numbers are 32-bit
 _f32 = torch.float32
 
 
@@ -44,18 +45,27 @@ def check_caches(k: torch.Tensor, v: torch.Tensor, B: int, Hkv: int, D: int, dty
         "caches must have 16-byte rows: unit stride in head_dim, other strides multiples of 8 elements, a 16-byte aligned base"
     if block_table is None:
         assert shape[0] >= B, "dense caches must be [bsz, num_kv_heads, ctx, head_dim]"
-        return kr, vr, shape[2], 0, 0, 0, 0
+        return kr, vr, min(shape[2], _MOST_ROWS), 0, 0, 0, 0
     page = shape[2]
     assert page % 64 == 0 and page > 0, "page_size must be a multiple of 64"
-    assert block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.get_device() == dev
     rows, width = block_table.shape
-    stride, one = block_table.stride()
-    assert rows == B and (one == 1 or width <= 1), "block_table must be [bsz, max_pages] int32 on the caches' device, unit stride along a row"
-    return kr, vr, width * page, block_table.data_ptr(), stride, page, shape[0]
+    assert rows == B, "block_table must be [bsz, max_pages]"
+    return kr, vr, min(width * page, _MOST_ROWS), block_table.data_ptr(), block_table.stride(0), page, shape[0]
+
+
+def table_of(block_table: Optional[torch.Tensor], caches: torch.Tensor) -> Optional[torch.Tensor]:
+    """The table as the kernels read it: int32, unit stride along a row, on the caches' device."""
+    if block_table is None:
+        return None
+    assert block_table.dtype in _LEN and block_table.dim() == 2, "block_table must be [bsz, max_pages] int32"
+    if block_table.dtype is not torch.int32 or block_table.get_device() != caches.get_device() or block_table.stride(1) != 1:
+        block_table = block_table.to(device=caches.device, dtype=torch.int32).contiguous()
+    return block_table
 
 
 def check_in_place(k: torch.Tensor, v: torch.Tensor, kr, vr, kv_seq_len: torch.Tensor, B: int) -> None:
     """kr, vr: the caches' pointers and strides."""
+    assert kr[0] != vr[0], "k_cache and v_cache are updated in place and must be two tensors"
     assert (0 not in kr or not _overlaps(k)) and (0 not in vr or not _overlaps(v)), "caches are updated in place and must not be expanded"
     assert B <= 1 or kv_seq_len.stride(0) == 1, "kv_seq_len is updated in place and must be contiguous"
 
@@ -88,6 +98,7 @@ def _decode(q, k, v, kv_seq_len, block_table, max_seq_len_in_batch, sm_scale, kv
     assert D in _HEAD_DIMS and code is not None, "q must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
     assert G >= 1 and H % G == 0, "num_heads must be a multiple of kv_group_num"
     Hkv = H // G
+    block_table = table_of(block_table, k)
     kr, vr, ctx, table, table_sb, page, n_pages = check_caches(k, v, B, Hkv, D, dt, dev, block_table)
     is64 = check_lengths(kv_seq_len, B, dev)
     if max_seq_len_in_batch is not None:
@@ -216,6 +227,7 @@ def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: i
     B = kv_seq_len.size(0)
     _, Hkv, _, D = k_cache.shape
     assert D in _HEAD_DIMS, "head_dim must be 32, 64, 128 or 256"
+    block_table = table_of(block_table, k_cache)
     kr, vr, ctx, table, table_sb, page, n_pages = check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
     is64 = check_lengths(kv_seq_len, B, dev)
     check_in_place(k_cache, v_cache, kr, vr, kv_seq_len, B)

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import launch, pack_rotary, rows_of
-from .decode import _DT, _HEAD_DIMS, _LEN, check_caches, check_in_place, check_lengths
+from .decode import _DT, _HEAD_DIMS, _LEN, check_caches, check_in_place, check_lengths, table_of
 
 _LAYOUT = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
 
@@ -164,6 +164,7 @@ def append_tokens(k_cache, v_cache, q, k, v, kv_seq_len, *, inv_freq: Optional[t
     code = _DT.get(dt)
     assert code is not None and D in _HEAD_DIMS, "k must be fp16 or bf16 with head_dim 32, 64, 128 or 256"
     assert k.get_device() == dev and v.get_device() == dev and v.dtype is dt and v.shape == k.shape, "k and v must be alike, on the caches' device"
+    block_table = table_of(block_table, k_cache)
     kc, vc, ctx, table, table_sb, page, n_pages = check_caches(k_cache, v_cache, B, Hkv, D, dt, dev, block_table)
     len64 = check_lengths(kv_seq_len, B, dev)
     check_in_place(k_cache, v_cache, kc, vc, kv_seq_len, B)

@@ -197,6 +197,31 @@ def test_captured_calls_follow_the_lengths():
 
 
 @pytest.mark.gpu
+def test_tables_and_lengths_of_other_kinds():
+    """int64 and strided tables, strided lengths, caches longer than the batch, a bound on the lengths."""
+    import flash_tree_attn_b200 as fta
+
+    torch.manual_seed(4)
+    k, v = (torch.randn(6, 2, 64, 64, device="cuda").half() for _ in "kv")
+    q = torch.randn(2, 4, 1, 64, device="cuda").half()
+    table = torch.tensor([[4, 1, 0], [2, 5, 3]], dtype=torch.int32, device="cuda")
+    n = torch.tensor([150, 70], device="cuda")
+    want = fta.decode_attention_paged(q, k, v, table, n, kv_group_num=2)
+    strided = torch.zeros(2, 6, dtype=torch.int32, device="cuda")
+    strided[:, ::2] = table
+    two = torch.zeros(4, dtype=torch.int64, device="cuda")
+    two[::2] = n
+    for t, lens in ((table.long(), n), (strided[:, ::2], n), (table.cpu(), n), (table, two[::2])):
+        assert torch.equal(fta.decode_attention_paged(q, k, v, t, lens, kv_group_num=2), want)
+    dense = fta.decode_attention(q, k, v, torch.tensor([64, 3], device="cuda"), kv_group_num=2)
+    assert torch.equal(fta.decode_attention(q, k, v, torch.tensor([200, 3], device="cuda"), kv_group_num=2), dense)  # never past the cache
+    bound = fta.decode_attention(q, k, v, torch.tensor([20, 3], device="cuda"), kv_group_num=2)
+    assert torch.equal(fta.decode_attention(q, k, v, torch.tensor([64, 3], device="cuda"), kv_group_num=2, max_seq_len_in_batch=20), bound)
+    none = fta.decode_attention(q, k, v, torch.tensor([-5, 0], device="cuda"), kv_group_num=2)
+    assert not none.any()
+
+
+@pytest.mark.gpu
 def test_page_outside_the_pool_takes_its_rows_out():
     import flash_tree_attn_b200 as fta
 

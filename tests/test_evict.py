@@ -127,10 +127,13 @@ def test_python_refusals():
 
     k = torch.zeros(2, 2, 64, 64, device="cuda", dtype=torch.float16)
     w, n = torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
-    fta.evict_rows(k, k.clone(), n, w, 4, 2)
-    for a in ((k, k, n, w, 0, 0), (k, k, n, w, 4, 5), (k, k, n, w, 4, -1), (k, k, n.float(), w, 4, 2), (k, k, n, w.half(), 4, 2), (k, k, n, w[..., :63], 4, 2),
-              (k, k[..., :32], n, w, 4, 2), (k.float(), k.float(), n, w, 4, 2), (k, k, n, w[:, :1].expand(2, 2, 64), 4, 2),
-              (k[:1].expand(2, 2, 64, 64), k, n, w, 4, 2), (k, k, torch.zeros(4, dtype=torch.int32, device="cuda")[::2], w, 4, 2)):
+    v = k.clone()
+    fta.evict_rows(k, v, n, w, 4, 2)
+    with pytest.raises(AssertionError, match="two tensors"):
+        fta.evict_rows(k, k, n, w, 4, 2)
+    for a in ((k, v, n, w, 0, 0), (k, v, n, w, 4, 5), (k, v, n, w, 4, -1), (k, v, n.float(), w, 4, 2), (k, v, n, w.half(), 4, 2), (k, v, n, w[..., :63], 4, 2),
+              (k, v[..., :32], n, w, 4, 2), (k.float(), v.float(), n, w, 4, 2), (k, v, n, w[:, :1].expand(2, 2, 64), 4, 2),
+              (k[:1].expand(2, 2, 64, 64), v, n, w, 4, 2), (k, v, torch.zeros(4, dtype=torch.int32, device="cuda")[::2], w, 4, 2)):
         with pytest.raises(AssertionError):
             fta.evict_rows(*a)
     with pytest.raises(RuntimeError, match="CUDA"):

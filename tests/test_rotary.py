@@ -254,14 +254,17 @@ def test_python_refusals():
                   ((x, x, pos, f), dict(layout="other")), ((x, x, pos, f), dict(offsets=n)), ((x[..., :48], None, pos, f), {})):
         with pytest.raises(AssertionError):
             fta.apply_rotary(*a, **kw)
-    fta.append_tokens(cache, cache.clone(), x, x, x, n)
-    for a, kw in (((cache[..., :32], cache, x, x, x, n), {}), ((cache[:1], cache[:1], x, x, x, n), {}), ((cache, cache, x, x, x, n.float()), {}),
-                  ((cache, cache, x, x, x[:, :1], n), {}), ((cache[:1].expand(2, 2, 64, 64), cache, x, x, x, n), {}),
-                  ((cache.bfloat16(), cache.bfloat16(), x, x, x, n), {}), ((cache, cache, x, x, x, torch.zeros(4, dtype=torch.int32, device="cuda")[::2]), {}),
-                  ((cache, cache, x[:, :, :1], x, x, n), {}), ((cache, cache, x, x, x, n), dict(block_table=torch.zeros(2, 1, device="cuda")))):
+    other = cache.clone()
+    fta.append_tokens(cache, other, x, x, x, n)
+    with pytest.raises(AssertionError, match="two tensors"):
+        fta.append_tokens(cache, cache, x, x, x, n)
+    for a, kw in (((cache[..., :32], other, x, x, x, n), {}), ((cache[:1], other[:1], x, x, x, n), {}), ((cache, other, x, x, x, n.float()), {}),
+                  ((cache, other, x, x, x[:, :1], n), {}), ((cache[:1].expand(2, 2, 64, 64), other, x, x, x, n), {}),
+                  ((cache.bfloat16(), other.bfloat16(), x, x, x, n), {}), ((cache, other, x, x, x, torch.zeros(4, dtype=torch.int32, device="cuda")[::2]), {}),
+                  ((cache, other, x[:, :, :1], x, x, n), {}), ((cache, other, x, x, x, n), dict(block_table=torch.zeros(2, 1, device="cuda")))):
         with pytest.raises(AssertionError):
             fta.append_tokens(*a, **kw)
     with pytest.raises(RuntimeError, match="CUDA"):
         fta.apply_rotary(x.cpu(), None, pos.cpu(), f.cpu())
     with pytest.raises(RuntimeError, match="CUDA"):
-        fta.append_tokens(cache.cpu(), cache.cpu(), x.cpu(), x.cpu(), x.cpu(), n.cpu())
+        fta.append_tokens(cache.cpu(), other.cpu(), x.cpu(), x.cpu(), x.cpu(), n.cpu())
