@@ -2,6 +2,9 @@
 
     from flash_tree_attn_b200 import flash_decoding_attention
 
+Beside it the other operators of a decoding loop: `decode_attention(_paged)`, `append_tokens`, `apply_rotary`,
+`evict_rows`, `commit_accepted`, `token_logprobs`, and a layer that uses them, `TreeVerifyAttention`.
+
 The arithmetic lives in libfta.so (hand-written sm_100a CUDA behind the C ABI of
 include/fta.h); build it with `python -m flash_tree_attn_b200.build`.
 """

@@ -251,7 +251,7 @@ def rows_of(t):
     return None if d != 1 or (a | b | c) & 7 or ptr & 15 else (ptr, a, b, c)
 
 
-_current_device = torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 

@@ -1,10 +1,12 @@
 /*
  * fta.h — C ABI of the B200 tree-attention decode library (libfta.so).
  *
- * One operator is exported: the tree-attention verification step of speculative
+ * The main operator is the tree-attention verification step of speculative
  * decoding.  Q tree queries per (sequence, head) attend densely to a right-padded
  * per-sequence KV cache of kv_seq_len[b] rows and, under an additive [Q,Q] mask, to
- * the Q new tree tokens; both parts are folded into one softmax.
+ * the Q new tree tokens; both parts are folded into one softmax.  Beside it stand the
+ * other operators of a decoding loop: accept/commit, attention of one new token, rotary
+ * positions and the cache append, eviction, token log probabilities.
  *
  * The entry points replace, for a caller that binds native code, the body of the
  * reference's only public function
