@@ -5,16 +5,32 @@
 // w_r += sum_h 2^(s_hr - LSE_h) from the scores stage 1 kept, so K is not read a second time
 // (4 G bytes a row instead of 2 D).
 //
-// grid = (B * Hkv, chunks of the cache's length): every block of a (sequence, KV head) works the
-// heads' LSEs out for itself, chunk 0 joins the outputs as well.
+// grid = (B * Hkv, max(shares, chunks of the cache's length)).  The group's heads are dealt out to the first
+// `shares` blocks of a KV head, and the pieces of a head to the block's warps where it has fewer heads
+// than warps: a few long units have up to a hundred pieces each.  With row weights every block works
+// all heads' LSEs out for itself and has a chunk of rows.
 #include "fta_token.cuh"
 
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 
-__global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenParams p, const FtaGeom g, const int chunk_rows) {
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+__global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenParams p, const FtaGeom g, const int shares, const int chunk_rows) {
   __shared__ float s_lse[FTA_MAX_GROUP];
+  __shared__ __align__(16) float s_o[kWarps][128];
+  __shared__ float s_top[kWarps], s_sum[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / p.Hkv, kvh = blockIdx.x - b * p.Hkv;
   const int G = p.H / p.Hkv, lanes = g.lanes > 0 ? g.lanes : 1;
@@ -30,62 +46,98 @@ __global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenP
 
   const int L = fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx);
   const int row0 = blockIdx.y * chunk_rows;
-  if (blockIdx.y > 0 && row0 >= L) return;
+  // {pieces, first group of blocks} of head hh's unit
+  auto pieces_of = [&](int hh) {
+    const int2 d = desc[(long long)b * g.U + kvh * g.n_gt + hh / g.R];  // asked for together with the length, which
+    return L > 0 ? d : make_int2(0, 0);                                 // says whether it was written
+  };
+  // row of piece i of head hh among the partial rows
+  auto slot = [&](int hh, int first, int i) {
+    const int lane_of = g.lanes > 1 ? hh / g.R : 0;
+    return ((long long)2 * ((first + i) * lanes + lane_of) + (i == 0 ? 1 : 0)) * g.R + hh % g.R;
+  };
 
-  for (int hh = warp; hh < G; hh += kThreads / 32) {
-    const int gt = hh / g.R, r = hh - gt * g.R, h = kvh * G + hh;
-    const int j = kvh * g.n_gt + gt;
-    float total = -INFINITY;
-    int2 d = desc[(long long)b * g.U + j];  // asked for together with the length, which says whether it was written
-    if (L == 0) d = make_int2(0, 0);
-    if (d.x == 1) {  // stage 1 wrote the rows itself
-      if (weights) total = lse2[(long long)b * p.H + h];
-    } else if (d.x > 1) {
-      const int lane_of = g.lanes > 1 ? gt : 0;
-      // slot of piece i in units of rows of D: lane i holds the LSE of pieces i, i + 32, ...
-      auto slot = [&](int i) { return ((long long)2 * ((d.y + i) * lanes + lane_of) + (i == 0 ? 1 : 0)) * g.R + r; };
-      const float mine = lane < d.x ? part_l[slot(lane)] : -INFINITY;
-      float top = mine, sum = 0.f;
-      for (int i = lane + 32; i < d.x; i += 32) top = fmaxf(top, part_l[slot(i)]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float base = top == -INFINITY ? 0.f : top;
-      const float w0 = fta_exp2(mine - base);  // NaN stays in sight here
-      sum = w0;
-      for (int i = lane + 32; i < d.x; i += 32) sum += fta_exp2(part_l[slot(i)] - base);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      total = sum == 0.f ? -INFINITY : base + fta_log2(sum);
-      if (blockIdx.y == 0) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        for (int c = 0; c < p.D; c += 128) {
-          const int c4 = c + lane * 4;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i0 = 0; i0 < d.x; i0 += 8) {  // eight pieces' loads go out together
+  if ((int)blockIdx.y < shares) {
+    const int heads = (G - 1 - (int)blockIdx.y) / shares + 1, columns = p.D > 128 ? 2 : 1;  // blockIdx.y < shares <= G
+    const int tasks = heads * columns;
+    const int team = tasks > 4 ? 1 : tasks > 2 ? 2 : tasks > 1 ? 4 : 8;  // warps per task
+    for (int t0 = 0; t0 < tasks; t0 += kWarps / team) {
+      const int t = t0 + warp / team, member = warp % team;
+      const int hh = blockIdx.y + shares * (t / columns), h = kvh * G + hh, c4 = (t % columns) * 128 + lane * 4;
+      const bool live = t < tasks, inside = c4 < p.D;
+      const int2 d = live ? pieces_of(hh) : make_int2(1, 0);
+      float top = -INFINITY, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (d.x > 1) {
+        for (int i0 = member; i0 < d.x; i0 += 32 * team) {  // lane j has the LSE of piece i0 + team j
+          const int i = i0 + team * lane, count = min(32, fta_cdiv(d.x - i0, team));
+          const float l = i < d.x ? part_l[slot(hh, d.y, i)] : -INFINITY;
+          const float now = fmaxf(top, warp_max(l)), base = now == -INFINITY ? 0.f : now;
+          const float keep = fta_exp2(top - base), w = fta_exp2(l - base);  // NaN stays in sight in w
+          acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+          sum = sum * keep + warp_sum(w);
+          top = now;
+          for (int j0 = 0; j0 < count; j0 += 8) {  // eight pieces' loads go out together
             float4 x[8];
-            float w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              x[u] = j0 + u < count && inside ? *reinterpret_cast<const float4*>(part_o + slot(hh, d.y, i0 + team * (j0 + u)) * p.D + c4)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-              const int i = i0 + u;
-              w[u] = i0 < 32 ? __shfl_sync(0xffffffffu, w0, i & 31) : i < d.x ? fta_exp2(part_l[slot(i)] - base) : 0.f;
-              x[u] = i < d.x && c4 < p.D ? *reinterpret_cast<const float4*>(part_o + slot(i) * p.D + c4) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              acc.x += w[u] * x[u].x; acc.y += w[u] * x[u].y; acc.z += w[u] * x[u].z; acc.w += w[u] * x[u].w;
+              const float f = __shfl_sync(0xffffffffu, w, (j0 + u) & 31);
+              acc.x += f * x[u].x; acc.y += f * x[u].y; acc.z += f * x[u].z; acc.w += f * x[u].w;
             }
           }
-          if (c4 < p.D) fta_store4(p.out, p.dtype, b * p.o_sb + h * p.o_sh + c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
         }
-        if (lane == 0 && p.lse) p.lse[b * p.l_sb + h] = total * FTA_LN2;
       }
-    } else if (blockIdx.y == 0) {  // no rows
-      for (int c4 = lane * 4; c4 < p.D; c4 += 128) fta_store4(p.out, p.dtype, b * p.o_sb + h * p.o_sh + c4, make_float4(0.f, 0.f, 0.f, 0.f));
-      if (lane == 0 && p.lse) p.lse[b * p.l_sb + h] = -INFINITY;
+      if (team > 1) {
+        *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
+        if (lane == 0) { s_top[warp] = top; s_sum[warp] = sum; }
+        __syncthreads();
+        if (member == 0) {
+          const float mine = lane < team ? s_top[warp + lane] : -INFINITY;
+          top = warp_max(mine);
+          const float base = top == -INFINITY ? 0.f : top;
+          sum = 0.f;
+          acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int m = 0; m < team; ++m) {
+            const float f = fta_exp2(s_top[warp + m] - base);
+            const float4 x = *reinterpret_cast<const float4*>(&s_o[warp + m][lane * 4]);
+            acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+            sum += f * s_sum[warp + m];
+          }
+        }
+        __syncthreads();
+      }
+      if (live && member == 0 && d.x != 1) {  // 1: stage 1 wrote the row itself; 0: no rows, zeros
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (inside)
+          fta_store4(p.out, p.dtype, b * p.o_sb + h * p.o_sh + c4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (c4 == 0 && p.lse) p.lse[b * p.l_sb + h] = sum == 0.f ? -INFINITY : (top + fta_log2(sum)) * FTA_LN2;
+      }
     }
-    if (weights && lane == 0) s_lse[hh] = total;
   }
-  if (!weights) return;
+  if (!weights || row0 >= L) return;
+
+  for (int hh = warp; hh < G; hh += kWarps) {
+    const int2 d = pieces_of(hh);
+    float total = -INFINITY;
+    if (d.x == 1) {
+      total = lse2[(long long)b * p.H + kvh * G + hh];
+    } else {
+      float l[4], top = -INFINITY, sum = 0.f;
+      for (int i0 = 0; i0 < d.x; i0 += 128) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l[u] = i0 + 32 * u + lane < d.x ? part_l[slot(hh, d.y, i0 + 32 * u + lane)] : -INFINITY;
+        const float now = fmaxf(top, warp_max(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])))), base = now == -INFINITY ? 0.f : now;
+        sum = sum * fta_exp2(top - base) + warp_sum(fta_exp2(l[0] - base) + fta_exp2(l[1] - base) + fta_exp2(l[2] - base) + fta_exp2(l[3] - base));
+        top = now;
+      }
+      total = sum == 0.f ? -INFINITY : top + fta_log2(sum);
+    }
+    if (lane == 0) s_lse[hh] = total;
+  }
   __syncthreads();
   // A thread has four consecutive rows and asks for eight heads' scores of them together: the loop waits
   // for memory and for nothing else.
@@ -237,7 +289,10 @@ extern "C" int fta_decode_token(const FtaTokenParams* p, void* stream) {
   if (e != cudaSuccess) return fta_cuda_fail(e);
   if (g.family == 1) return FTA_OK;
   const int chunk = 4 * kThreads;
-  const dim3 grid(p->B * p->Hkv, weights ? (p->ctx + chunk - 1) / chunk + (p->ctx == 0) : 1);
-  e = fta_launch_after(token_join_kernel, grid, kThreads, 0, st, 1, *p, g, chunk);
+  const int chunks = weights ? fta_cdiv(p->ctx, chunk) : 0;
+  // a block per head where there are few KV heads: then a unit has many pieces
+  const int shares = p->B * p->Hkv < 148 ? p->H / p->Hkv : 1;
+  const dim3 grid(p->B * p->Hkv, shares > chunks ? shares : chunks);
+  e = fta_launch_after(token_join_kernel, grid, kThreads, 0, st, 1, *p, g, shares, chunk);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }
