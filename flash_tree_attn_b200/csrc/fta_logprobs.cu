@@ -35,14 +35,15 @@ namespace {
 
 constexpr int kChunks = 8;        // 16-byte chunks per thread and round
 constexpr int kMostBlocks = 8;    // of a cluster, so of a row
-// 256 threads a row, 4 blocks an SM: one computes while the others' chunks arrive.  64 threads, 16 blocks an
-// SM, for many rows of a few thousand logits: such a block's time is its barriers and latencies.
+// 256 threads a row, 4 blocks an SM: one computes while the others' chunks arrive.  64 threads, or a single
+// warp, for many rows of a few thousand logits: such a block's time is its barriers and latencies, and
+// more of them fit an SM (26867 rows of 601: 64 threads 37 us, a warp 29).
 template <int THREADS> struct Cfg {
   static constexpr int kWarps = THREADS / 32;
   static constexpr int kBlocks = 1024 / THREADS;                   // per SM
-  static constexpr int kListedChunks = THREADS == 64 ? 128 : 256;
+  static constexpr int kListedChunks = THREADS == 32 ? 64 : THREADS == 64 ? 128 : 256;
   static constexpr int kListed = 8 * kListedChunks;                // elements ranked by counting
-  static constexpr int kPending = THREADS == 64 ? 0 : 64;          // listed chunks that may wait for the next round
+  static constexpr int kPending = THREADS < 256 ? 0 : 64;          // listed chunks that may wait for the next round
   static constexpr int kMostRounds = 32;                           // largest q: a warp's lanes
 };
 
@@ -495,8 +496,13 @@ int run_with(const FtaLogprobParams& p, cudaStream_t st) {
 
 template <typename T>
 int run(const FtaLogprobParams& p, cudaStream_t st) {
-  const bool small = p.vocab / Vec<T>::n <= 64 * kChunks && p.rows > 148 * 4;
-  return small ? run_with<T, 64>(p, st) : run_with<T, 256>(p, st);
+  // The first round's bound is loose where k comes near the number of lanes (it is the k-th largest lane
+  // maximum at best): a warp's 64 chunks then hold twice or three times k for k up to 16, two warps' 128 for k
+  // up to 40; beyond, the lists would overflow, unless they hold all of a row, and the exact bound be searched.
+  const int chunks = p.vocab / Vec<T>::n;
+  if (p.rows > 148 * 4 && chunks <= 32 * kChunks && p.top_k <= 16) return run_with<T, 32>(p, st);
+  if (p.rows > 148 * 4 && chunks <= (p.top_k <= 40 ? 64 * kChunks : Cfg<64>::kListedChunks)) return run_with<T, 64>(p, st);
+  return run_with<T, 256>(p, st);
 }
 
 }  // namespace

@@ -44,7 +44,7 @@ def _tokens(rows, V, n, g, dtype=torch.int64):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,V,k", [(1, 1, 1), (3, 2, 2), (2, 7, 3), (5, 64, 64), (3, 100, 64), (2, 255, 5), (2, 2049, 20), (3, 4097, 64), (2, 16384, 1),
                                       (2, 32768, 33), (2, 32769, 64), (300, 1000, 8), (3, 50257, 20), (2, 128256, 5), (1, 262144, 64), (2, 300001, 10), (4, 5000, 0),
-                                      (700, 1000, 64), (601, 4095, 20), (601, 33, 5), (2, 16500, 64), (20, 56697, 64)])
+                                      (700, 1000, 64), (601, 4095, 20), (601, 33, 5), (601, 1, 1), (601, 2047, 16), (601, 257, 33), (601, 300, 64), (601, 1023, 64), (601, 1040, 64), (601, 4000, 40), (2, 16500, 64), (20, 56697, 64)])
 def test_matches_the_formula(dtype, rows, V, k):
     import flash_tree_attn_b200 as fta
 
@@ -71,8 +71,8 @@ def test_rows_that_start_anywhere(dtype, shift):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["equal", "two values", "masked", "all masked", "nan", "inf", "rising", "one high", "far", "lowest", "lowest and masked", "blocks"])
-@pytest.mark.parametrize("V,rows", [(50, 4), (3000, 4), (70001, 4), (2999, 601)])
-def test_rows_that_tie_or_are_masked(kind, V, rows):
+@pytest.mark.parametrize("V,rows,k", [(50, 4, 40), (3000, 4, 40), (70001, 4, 40), (2999, 601, 40), (2999, 601, 41), (1999, 601, 16), (301, 601, 3)])
+def test_rows_that_tie_or_are_masked(kind, V, rows, k):
     import flash_tree_attn_b200 as fta
 
     g = torch.Generator().manual_seed(V)
@@ -114,7 +114,7 @@ def test_rows_that_tie_or_are_masked(kind, V, rows):
             x = x / 4
         y = x.to(dtype).cuda()
         t = _tokens(rows, V, 2, g)
-        _check(y, t, 40, fta.token_logprobs(y, t, 40))
+        _check(y, t, k, fta.token_logprobs(y, t, k))
 
 
 @pytest.mark.gpu
