@@ -182,3 +182,56 @@ def test_children_of_a_tree():
     tree = fta.DraftTree(PARENTS, device="cpu")
     assert tree.children.tolist() == [[1, 2], [3, 4], [5, -1], [6, -1], [-1, -1], [-1, -1], [-1, -1]]
     assert tree.parent.tolist() == [0, 0, 0, 1, 1, 2, 3] and tree.slot.tolist() == [0, 0, 1, 0, 1, 0, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [None, 64])
+def test_hundreds_of_steps_without_a_synchronisation(page):
+    """Kernels are set up while the one before drains: steps queued without a pause, on two streams at once,
+    give the bits of steps that wait for one another."""
+    import flash_tree_attn_b200 as fta
+
+    B, H, Hkv, D = 3, 8, 2, 128
+    f, _ = fta.rotary_frequencies(64)
+    tree = fta.DraftTree(PARENTS)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    make = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()  # noqa: E731
+    prompt, steps = (make(B, Hkv, 500, D), make(B, Hkv, 500, D)), [tuple(make(B, h, 1, D) for h in (H, Hkv, Hkv)) for _ in range(4)]
+    draft = tuple(make(B, h, tree.Q, D) for h in (H, Hkv, Hkv))
+    head = make(H * D, 5000)
+    layers = [fta.TreeVerifyAttention(H, Hkv, D, B, 4096, torch.bfloat16, page_size=page, rotary=(f, "interleaved", 1.0), track_weights=True)
+              for _ in range(3)]
+    for layer in layers:
+        layer.load_prefix(*prompt, [500, 3, 77])
+    torch.cuda.synchronize()
+
+    def run(layer, wait):
+        seen = []
+        for i in range(60):
+            out = layer.decode(*steps[i % 4])
+            wait()
+            r = fta.token_logprobs(out.reshape(B, -1) @ head, top_k=5)
+            wait()
+            if i % 5 == 4:
+                verified = layer(*draft, tree.mask, depth=tree.depth)
+                wait()
+                ok = fta.greedy_node_ok(tree, verified.transpose(1, 2).reshape(B, tree.Q, -1) @ head, r.top_ids[:, :1].expand(B, tree.Q))
+                layer.commit(*fta.accept_longest_path(tree, ok))
+                wait()
+                seen.append(verified)
+            if i % 7 == 6:
+                seen.append(layer.evict(300, 40))
+                wait()
+            seen += [out, *r[1:]]
+        return seen
+
+    want = run(layers[0], torch.cuda.synchronize)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for layer, s in zip(layers[1:], streams):
+        with torch.cuda.stream(s):
+            got.append(run(layer, lambda: None))
+    torch.cuda.synchronize()
+    for layer, seen in zip(layers[1:], got):
+        assert all(torch.equal(a, b) for a, b in zip(seen, want))
+        for name in ("k_cache", "v_cache", "kv_seq_len", "row_weights", "next_position"):
+            assert torch.equal(getattr(layer, name), getattr(layers[0], name)), name
