@@ -52,6 +52,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+// The likeliest go by bits (`ordered`), so what is held against their bound as a float keeps subnormals
+// apart too: the compiler's own comparisons take them all for zero (--use_fast_math), and a guard that sees
+// equals where the bits differ would let more elements into the list than it holds.
+__device__ __forceinline__ bool below(float a, float b) {  // false where either is NaN
+  int y;
+  asm("{ .reg .pred p; setp.lt.f32 p, %1, %2; selp.s32 %0, 1, 0, p; }" : "=r"(y) : "f"(a), "f"(b));
+  return y != 0;
+}
+__device__ __forceinline__ bool at_most(float a, float b) {
+  int y;
+  asm("{ .reg .pred p; setp.le.f32 p, %1, %2; selp.s32 %0, 1, 0, p; }" : "=r"(y) : "f"(a), "f"(b));
+  return y != 0;
+}
+__device__ __forceinline__ float max_num(float a, float b) {  // a NaN stays out
+  float y;
+  asm("max.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // adds 2^d and 2^d d
 __device__ __forceinline__ void add_exp(float d, float& s, float& t) {
   const float e = fta_exp2(d);
@@ -116,16 +134,22 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// order of floats as unsigned integers; -0 and +0 alike, NaN on top; 0 is below every float
+// order of floats as unsigned integers; -0 and +0 alike, NaN on top; 0 is below every float.  The bits are moved
+// by hand: of plain casts around operations on the sign bit the compiler makes an absolute value and a
+// negation of floats, and those flush subnormals.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
+  uint32_t b;
+  asm("mov.b32 %0, %1;" : "=r"(b) : "f"(x));
   if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
   if (b == 0x80000000u) return b;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t k) {
   if (k == 0xffffffffu) return NAN;
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+  const uint32_t b = k & 0x80000000u ? k & 0x7fffffffu : ~k;
+  float x;
+  asm("mov.b32 %0, %1;" : "=f"(x) : "r"(b));
+  return x;
 }
 // one number that ranks by value, then by lower token
 __device__ __forceinline__ unsigned long long rank_key(uint32_t k, int token) {
@@ -176,7 +200,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
   constexpr int kRound = kThreads * kChunks, kWarps = Cfg<kThreads>::kWarps, kMostRounds = Cfg<kThreads>::kMostRounds;
   constexpr int kListedChunks = Cfg<kThreads>::kListedChunks, kPending = Cfg<kThreads>::kPending;
   // room for what waits from earlier rounds, a whole list, the row's edges, the likeliest so far, and zeros
-  __shared__ __align__(16) unsigned long long list[8 * kPending + Cfg<kThreads>::kListed + 2 * VE + FTA_MAX_TOP_K + 8];
+  constexpr int kRoom = 8 * kPending + Cfg<kThreads>::kListed + 2 * VE;
+  __shared__ __align__(16) unsigned long long list[kRoom + FTA_MAX_TOP_K + 8];
   __shared__ unsigned long long best[FTA_MAX_TOP_K];  // the likeliest so far, in order; 0: none
   __shared__ Sums s_sums;
   __shared__ float s_a[kWarps], s_b[kWarps], s_c[kWarps];
@@ -201,6 +226,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
                                            : (long long)reinterpret_cast<const int*>(p.tokens)[row * p.t_sr + i];
     inside = tok >= 0 && tok < p.vocab;
     return inside ? to_float(x[tok]) : -INFINITY;
+  };
+  // The counts that decide what is appended leave room for it; an index past the room is dropped all the same.
+  auto append = [&](uint32_t key, int token) {
+    const int to = atomicAdd(&s_listed, 1);
+    if (to < kRoom) list[to] = rank_key(key, token);
   };
   bool asked_inside = false;
   const float asked = block == 0 && tid < p.n_tokens ? logit_of(tid, asked_inside) : 0.f;
@@ -310,10 +340,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
     // list the chunks that reach the bound (NaN does)
     uint32_t reach = 0;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) reach |= top[c] < bound ? 0u : 1u << c;
+    for (int c = 0; c < kChunks; ++c) reach |= below(top[c], bound) ? 0u : 1u << c;
     uint32_t larger_than = 0;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) larger_than |= top[c] <= bound ? 0u : 1u << c;
+    for (int c = 0; c < kChunks; ++c) larger_than |= at_most(top[c], bound) ? 0u : 1u << c;
     while (reach != 0) {
       const int bit = __ffs(reach) - 1, c = bit * kThreads + tid;
       reach &= reach - 1;
@@ -322,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
       if (to < kListedChunks) s_where[to] = base + c;
       if ((larger_than >> bit) & 1) atomicAdd(&s_larger, 1);
     }
-    if (edge >= 0 && !(edge_logit < bound)) list[atomicAdd(&s_listed, 1)] = rank_key(ordered(edge_logit), edge);
+    if (edge >= 0 && !below(edge_logit, bound)) append(ordered(edge_logit), edge);
     __syncthreads();
     const int reached = s_n;
     if (round > 0 && round + 1 < rounds && base + kRound < total && reached <= kPending) {
@@ -334,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
     for (int i = tid; i < listed * VE; i += kThreads) {
       const int tok = start + s_where[i / VE] * VE + i % VE;
       const float v = to_float(x[tok]);
-      if (!(v < bound)) list[atomicAdd(&s_listed, 1)] = rank_key(ordered(v), tok);
+      if (!below(v, bound)) append(ordered(v), tok);
     }
     __syncthreads();
     if (over) {
@@ -354,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
       for (int i = lo + tid; i < hi; i += kThreads) {
         const uint32_t o = ordered(to_float(x[i]));
         if (o > key) {
-          list[atomicAdd(&s_listed, 1)] = rank_key(o, i);
+          append(o, i);
           ++larger;
         }
       }
@@ -371,13 +401,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
           before += w < warp ? (int)s_key[w] : 0;
           all += s_key[w];
         }
-        if (o == key && i < hi && before < wanted) list[atomicAdd(&s_listed, 1)] = rank_key(o, i);
+        if (o == key && i < hi && before < wanted) append(o, i);
         wanted -= all;
         __syncthreads();
       }
       __syncthreads();
     }
-    int n = s_listed;
+    int n = min(s_listed, kRoom);
     if (round > 0) {
       for (int i = tid; i < k; i += kThreads) list[n + i] = best[i];
       n += k;
@@ -393,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
     __syncthreads();
     pending = 0;
     // what comes later has to reach the k-th largest so far; a NaN there stays out of the comparison
-    if (best[k - 1] != 0) bound = fmaxf(bound, unordered((uint32_t)(best[k - 1] >> 32)));
+    if (best[k - 1] != 0) bound = max_num(bound, unordered((uint32_t)(best[k - 1] >> 32)));
   }
 
   // the block's sums, against its largest reference
