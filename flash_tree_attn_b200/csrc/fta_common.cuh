@@ -292,6 +292,7 @@ template <> struct FtaType<__half> {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
   static __device__ __forceinline__ __half from_float(float a) { return __float2half_rn(a); }
 };
 template <> struct FtaType<__nv_bfloat16> {
@@ -300,6 +301,7 @@ template <> struct FtaType<__nv_bfloat16> {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x)); }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float a) { return __float2bfloat16_rn(a); }
 };
 
