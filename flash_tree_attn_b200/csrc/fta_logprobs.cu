@@ -3,12 +3,13 @@
 //
 // With m the largest logit, s = sum e^(x - m) and t = sum e^(x - m) (x - m):
 //   lse = m + log s,  entropy = log s - t / s,  log p(token) = x[token] - lse.
-// Every term of t has the same sign, so the entropy loses nothing but in the last difference.
+// Every term of t has the same sign, s is 1 and more, and so both terms of the entropy are positive.
 //
 // What bounds it: the logits are read once; with 16-bit logits an SM gets about 12 elements a clock from
 // memory, so there is room for about 10 instructions an element, and 16 exponentials a clock.  So each
-// thread keeps sums of its own against a reference of its own, which moves only when a logit passes it
-// by 14 (in 32 bits a ratio of sums does not care), with 6 instructions an element: the exponent is
+// thread keeps sums of its own against its own largest logit so far, with 6 instructions an element (a
+// reference that lags behind would save a move a round, and make two large numbers of a peaked row's entropy,
+// whose difference then comes out below 0): the exponent is
 // x log2(e) - c, c = m log2(e) rounded, one fused multiply-add, and what the rounding of c shifts,
 // r = m log2(e) - c, is known exactly and taken out at the end.  Where |m| >= 30000 (logits masked with the
 // type's lowest value and nothing else) it is (x - m) log2(e), which cannot overflow.
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
   const float asked = block == 0 && tid < p.n_tokens ? logit_of(tid, asked_inside) : 0.f;
 
   // the thread's reference, its rounded log2(e) multiple, what that rounding shifts, and the sums
-  float m = -INFINITY, c2 = 0.f, r = 0.f, s = 0.f, t = 0.f, limit = -INFINITY;
+  float m = -INFINITY, c2 = 0.f, r = 0.f, s = 0.f, t = 0.f;
   bool near = true;
   float bound = -INFINITY;
   int pending = 0;  // listed chunks that wait
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
       }
     }
 
-    if (mine > limit) {
+    if (mine > m) {
       const float to2 = __fmul_rn(mine, FTA_LOG2E);
       near = fabsf(mine) < 30000.f;
       const float r_to = near ? fmaf(mine, FTA_LOG2E, -to2) : 0.f;
@@ -316,7 +317,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
       t = f == 0.f ? 0.f : f * (t + shift * s);
       s *= f;
       m = mine; c2 = to2; r = r_to;
-      limit = mine + 14.f;
     }
     if (mine != -INFINITY) {
       if (near) {
@@ -470,11 +470,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<kThreads>::kBlocks) logprob_kern
   }
   m = sums.m;
   s = sums.s;
-  const float log2_s = fta_log2(s);
-  const float log_s = log2_s * FTA_LN2;
+  // the largest logit's term is 1; roundings that take s below it, or t above 0, are put right (NaN stays)
+  const float rest = s < 1.f ? 0.f : s - 1.f;
+  const float log_s = log1pf(rest);
   if (tid == 0) {
+    const float mean = sums.t > 0.f ? 0.f : sums.t / s * FTA_LN2;
     p.lse[row] = s == 0.f ? -INFINITY : m + log_s;
-    p.entropy[row] = s == 0.f ? 0.f : (log2_s - sums.t / s) * FTA_LN2;
+    p.entropy[row] = s == 0.f ? 0.f : log_s - mean;
   }
   // (x - m) - log s: what m and lse have in common is not rounded
   auto log_p = [&](float v) { return s == 0.f || v == -INFINITY ? (s != s ? s : -INFINITY) : (v - m) - log_s; };
