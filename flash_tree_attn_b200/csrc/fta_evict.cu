@@ -25,6 +25,7 @@ constexpr int kKeys = 24 * 1024;  // rows whose weights fit the select block's s
 constexpr int kMove = 256;
 constexpr int kAhead = 3;         // rows per thread and chunk
 constexpr int kBins = 2048;
+constexpr int kMostRows = FTA_MAX_EVICT_ROWS;  // loops over rows are 32-bit and step past the end by up to 2^15
 
 // Weights are handled as their bits throughout: arithmetic would take the smallest ones for zeros.
 // Their order as unsigned integers; -0 and +0 alike, NaN on top.
@@ -273,6 +274,7 @@ bool rows16(const void* x, int64_t a, int64_t b, int64_t c) {
 extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
   if (!p || p->B <= 0 || p->Hkv <= 0 || p->ctx < 0 || p->budget <= 0 || p->recent < 0 || p->recent > p->budget) return FTA_E_BADARG;
   if (p->D != 32 && p->D != 64 && p->D != 128 && p->D != 256) return FTA_E_BADARG;
+  if (p->ctx > kMostRows || p->budget > kMostRows) return FTA_E_UNSUPPORTED;
   if (!p->k_cache || !p->v_cache || !p->kv_seq_len || !p->row_weights || !p->kept) return FTA_E_BADARG;
   if (!rows16(p->k_cache, p->k_sb, p->k_sh, p->k_st) || !rows16(p->v_cache, p->v_sb, p->v_sh, p->v_st)) return FTA_E_BADARG;
   if (p->block_table && (p->page_size < 1 || p->n_pages < 1 || p->bt_sb < 0 || (p->B > 1 && (long long)p->bt_sb * p->page_size < p->ctx)))

@@ -20,7 +20,7 @@ from ._lib import launch, pack_evict, pack_token, rows_of
 _DT = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _LEN = {torch.int32: 0, torch.int64: 1}  # -> is int64
 _HEAD_DIMS = (32, 64, 128, 256)
-_MOST_ROWS = 0x7fffff00  # of a sequence: row numbers are 32-bit
+_MOST_ROWS = 0x7fff0000  # of a sequence: row numbers are 32-bit, and loops over them step past the end
 _f32 = torch.float32
 
 
@@ -211,7 +211,7 @@ def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: i
         kv_seq_len: [bsz] int32/int64 on the device, becomes min(length, budget) in place.
         row_weights: [bsz, num_kv_heads, ctx] fp32 as decode_attention adds them up, updated in place:
             0 from the new length to the old one, so that appended rows start at 0.
-        budget, recent: 1 <= budget, 0 <= recent <= budget.
+        budget, recent: 1 <= budget <= 2^31 - 2^16, 0 <= recent <= budget.
 
     Returns kept [bsz, num_kv_heads, budget] int32, the old row of every row now in the cache (-1 past
     a shorter sequence's end).  Keys keep the rotary positions they were written with; a caller that
@@ -234,7 +234,7 @@ def evict_rows(k_cache, v_cache, kv_seq_len, row_weights, budget: int, recent: i
     assert row_weights.dim() == 3, "row_weights must be [bsz, num_kv_heads, ctx]"
     rw, rw_sb, rw_sh = check_weights(row_weights, B, Hkv, ctx, dev)
     budget, recent = int(budget), int(recent)
-    assert 1 <= budget <= 0x7fffffff and 0 <= recent <= budget, "1 <= budget and 0 <= recent <= budget"
+    assert 1 <= budget <= _MOST_ROWS and 0 <= recent <= budget, "1 <= budget <= 2^31 - 2^16 and 0 <= recent <= budget"
     kept = torch.empty(B, Hkv, budget, dtype=torch.int32, device=k_cache.device)
     if B and Hkv:
         launch(lib.fta_evict_rows, pack_evict(*kr, *vr, kv_seq_len.data_ptr(), table, table_sb, rw, rw_sb, rw_sh, kept.data_ptr(),

@@ -353,8 +353,9 @@ int fta_append_tokens(const FtaRotaryParams* p, void* stream);
  * old order, and their weights with them.  row_weights of rows [budget, L) become 0, K and V there
  * stay as they are.  kv_seq_len[b] becomes min(L, budget).  Other sequences are left alone.
  *   kept  [B, Hkv, budget] int32, contiguous: the old row of every new row, -1 past a sequence's end
- * A page outside [0, n_pages) is neither read nor written.
+ * A page outside [0, n_pages) is neither read nor written.  ctx and budget are at most FTA_MAX_EVICT_ROWS.
  */
+#define FTA_MAX_EVICT_ROWS 0x7fff0000
 typedef struct FtaEvictParams {
   void* k_cache;
   int64_t k_sb, k_sh, k_st;
