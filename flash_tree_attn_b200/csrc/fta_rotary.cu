@@ -71,9 +71,10 @@ __global__ void __launch_bounds__(kThreads, 8) rotary_kernel(const FtaRotaryPara
 
   const int L = APPEND ? fta_load_len(p.kv_seq_len, p.len_is_i64, b, p.ctx) : 0;
   if (APPEND && (int)threadIdx.x < TOK) {
-    const int row = L + i0 + (int)threadIdx.x;
+    const unsigned wide = (unsigned)L + i0 + threadIdx.x;  // a long cache and a long chunk: past 2^31, below 2^32
+    bool fits = wide < (unsigned)p.ctx;
+    const int row = fits ? (int)wide : 0;
     long long at = b, in = row;
-    bool fits = row >= 0 && row < p.ctx;
     if (p.block_table != nullptr && fits) {
       at = p.block_table[b * p.bt_sb + row / p.page_size];
       in = row % p.page_size;

@@ -29,3 +29,21 @@ def test_eviction_without_a_limit_is_refused_before_anything_is_allocated():
     assert torch.cuda.memory_allocated() == before and n.item() == 5
     fta.evict_rows(k, v, n, w, 64, 64)
     assert n.item() == 5
+
+
+@pytest.mark.gpu
+def test_append_of_a_chunk_whose_row_numbers_pass_32_bits():
+    """A table of 2^31 - 2^16 rows, all of one page; the chunk starts two rows before the end and is longer than
+    what is left below 2^31.  Two rows are written, the others dropped."""
+    import flash_tree_attn_b200 as fta
+
+    Q, D = 70000, 32
+    table = torch.zeros(1, MOST // 64 + 5, dtype=torch.int32, device="cuda")
+    kc, vc = (torch.zeros(1, 1, 64, D, device="cuda", dtype=torch.float16) for _ in "kv")
+    k = torch.randn(1, 1, Q, D, device="cuda").half()
+    v = torch.randn(1, 1, Q, D, device="cuda").half()
+    n = torch.tensor([MOST - 2], dtype=torch.int64, device="cuda")
+    fta.append_tokens(kc, vc, k, k, v, n, block_table=table)
+    assert n.item() == MOST
+    for cache, x in ((kc, k), (vc, v)):
+        assert torch.equal(cache[0, 0, 62:], x[0, 0, :2]) and not cache[0, 0, :62].any()
