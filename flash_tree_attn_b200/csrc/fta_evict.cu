@@ -25,7 +25,7 @@ constexpr int kKeys = 24 * 1024;  // rows whose weights fit the select block's s
 constexpr int kMove = 256;
 constexpr int kAhead = 3;         // rows per thread and chunk
 constexpr int kBins = 2048;
-constexpr int kMostRows = FTA_MAX_EVICT_ROWS;  // loops over rows are 32-bit and step past the end by up to 2^15
+constexpr int kMostRows = FTA_MAX_ROWS;  // loops over rows are 32-bit and step past the end by up to 2^15
 
 // Weights are handled as their bits throughout: arithmetic would take the smallest ones for zeros.
 // Their order as unsigned integers; -0 and +0 alike, NaN on top.

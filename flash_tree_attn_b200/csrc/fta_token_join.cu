@@ -145,29 +145,32 @@ __global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenP
   const float* scores = reinterpret_cast<const float*>(wsb + ws.scores) + ((long long)b * p.H + kvh * G) * pitch;
   float* out = p.row_weights + b * p.rw_sb + kvh * p.rw_sh;
   const int first = p.window > 0 ? max(0, L - p.window) : 0;
-  const int row = row0 + 4 * (int)threadIdx.x;
-  if (row + 3 < first || row >= L) return;
-  float old[4], w[4] = {0.f, 0.f, 0.f, 0.f};
+  const int end = min(L, row0 + chunk_rows);
+#pragma unroll 1
+  for (int row = row0 + 4 * (int)threadIdx.x; row < end; row += 4 * kThreads) {
+    if (row + 3 < first) continue;
+    float old[4], w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) old[e] = row + e >= first && row + e < L ? out[row + e] : 0.f;
-  for (int h0 = 0; h0 < G; h0 += 8) {
-    float4 x[8];
+    for (int e = 0; e < 4; ++e) old[e] = row + e >= first && row + e < L ? out[row + e] : 0.f;
+    for (int h0 = 0; h0 < G; h0 += 8) {
+      float4 x[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (h0 + u < G) x[u] = __ldcs(reinterpret_cast<const float4*>(scores + (h0 + u) * pitch + row));
+      for (int u = 0; u < 8; ++u)
+        if (h0 + u < G) x[u] = __ldcs(reinterpret_cast<const float4*>(scores + (h0 + u) * pitch + row));
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float total = h0 + u < G ? s_lse[h0 + u] : -INFINITY;
-      if (total == -INFINITY) continue;
-      w[0] += fta_exp2(x[u].x - total);
-      w[1] += fta_exp2(x[u].y - total);
-      w[2] += fta_exp2(x[u].z - total);
-      w[3] += fta_exp2(x[u].w - total);
+      for (int u = 0; u < 8; ++u) {
+        const float total = h0 + u < G ? s_lse[h0 + u] : -INFINITY;
+        if (total == -INFINITY) continue;
+        w[0] += fta_exp2(x[u].x - total);
+        w[1] += fta_exp2(x[u].y - total);
+        w[2] += fta_exp2(x[u].z - total);
+        w[3] += fta_exp2(x[u].w - total);
+      }
     }
-  }
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (row + e >= first && row + e < L) out[row + e] = old[e] + w[e];
+    for (int e = 0; e < 4; ++e)
+      if (row + e >= first && row + e < L) out[row + e] = old[e] + w[e];
+  }
 }
 
 template <typename F>
@@ -187,7 +190,7 @@ int check_sizes(const FtaTokenParams* p) {
   if (p->D != 32 && p->D != 64 && p->D != 128 && p->D != 256) return FTA_E_BADARG;
   if (p->dtype != FTA_DTYPE_F16 && p->dtype != FTA_DTYPE_BF16) return FTA_E_BADARG;
   if (p->grid_override < 0) return FTA_E_BADARG;
-  if (p->B > FTA_MAX_BATCH || p->H / p->Hkv > FTA_MAX_GROUP) return FTA_E_UNSUPPORTED;
+  if (p->B > FTA_MAX_BATCH || p->H / p->Hkv > FTA_MAX_GROUP || p->ctx > FTA_MAX_ROWS) return FTA_E_UNSUPPORTED;
   return FTA_OK;
 }
 
@@ -288,7 +291,8 @@ extern "C" int fta_decode_token(const FtaTokenParams* p, void* stream) {
   cudaError_t e = (cudaError_t)token_variant(*p, [&](auto launch) { return (int)launch(*p, g, st, 0, nullptr); });
   if (e != cudaSuccess) return fta_cuda_fail(e);
   if (g.family == 1) return FTA_OK;
-  const int chunk = 4 * kThreads;
+  int chunk = 4 * kThreads;
+  while (weights && fta_cdiv(p->ctx, chunk) > 65535) chunk *= 2;  // a grid's second dimension ends there
   const int chunks = weights ? fta_cdiv(p->ctx, chunk) : 0;
   // a block per head where there are few KV heads: then a unit has many pieces
   const int shares = p->B * p->Hkv < 148 ? p->H / p->Hkv : 1;

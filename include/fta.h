@@ -246,6 +246,8 @@ typedef struct FtaCommitParams {
 
 int fta_commit_accepted(const FtaCommitParams* p, void* stream);
 
+#define FTA_MAX_ROWS 0x7fff0000 /* of a sequence: loops over rows are 32-bit and step past the end */
+
 /*
  * Attention of ONE new token per sequence over the cache (the decoding step without a draft tree).
  * The new token's own key and value are already in the cache (fta_append_tokens), so that
@@ -256,7 +258,7 @@ int fta_commit_accepted(const FtaCommitParams* p, void* stream);
  *   row_weights  optional fp32 [B, Hkv, ctx], unit stride along ctx: row r of KV head kvh gains the
  *                softmax weights that the group's G query heads gave it (updated in place, by one
  *                thread per row in a fixed order: equal inputs give equal bits)
- * An empty sequence gives out = 0, lse = -inf.  A page index outside [0, n_pages) takes the rows
+ * ctx is at most FTA_MAX_ROWS.  An empty sequence gives out = 0, lse = -inf.  A page index outside [0, n_pages) takes the rows
  * of that page out of the attention; nothing outside the pool is read.
  */
 typedef struct FtaTokenParams {
@@ -353,9 +355,8 @@ int fta_append_tokens(const FtaRotaryParams* p, void* stream);
  * old order, and their weights with them.  row_weights of rows [budget, L) become 0, K and V there
  * stay as they are.  kv_seq_len[b] becomes min(L, budget).  Other sequences are left alone.
  *   kept  [B, Hkv, budget] int32, contiguous: the old row of every new row, -1 past a sequence's end
- * A page outside [0, n_pages) is neither read nor written.  ctx and budget are at most FTA_MAX_EVICT_ROWS.
+ * A page outside [0, n_pages) is neither read nor written.  ctx and budget are at most FTA_MAX_ROWS.
  */
-#define FTA_MAX_EVICT_ROWS 0x7fff0000
 typedef struct FtaEvictParams {
   void* k_cache;
   int64_t k_sb, k_sh, k_st;
