@@ -27,6 +27,14 @@ __device__ __forceinline__ float warp_sum(float x) {
   return x;
 }
 
+// eviction orders weights by their bits, so a row that gains nothing keeps its own, subnormal ones too, which
+// the compiler's addition takes for zero (--use_fast_math)
+__device__ __forceinline__ float add_kept(float a, float b) {
+  float y;
+  asm("add.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 __global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenParams p, const FtaGeom g, const int shares, const int chunk_rows) {
   __shared__ float s_lse[FTA_MAX_GROUP];
   __shared__ __align__(16) float s_o[kWarps][128];
@@ -169,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_join_kernel(const FtaTokenP
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (row + e >= first && row + e < L) out[row + e] = old[e] + w[e];
+      if (row + e >= first && row + e < L) out[row + e] = add_kept(old[e], w[e]);
   }
 }
 

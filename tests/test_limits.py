@@ -97,3 +97,21 @@ def test_row_weights_of_a_cache_of_many_chunks():
         d = 40 * 2.0 ** -24 * ora["score"] + 2.0 ** -20
         assert ((w[..., L - 300: L].double().cpu() - ora["weights"]).abs() <= ora["weights"] * (3 * d + 2.0 ** -15)).all()
         assert not w[..., : L - 300].any() and not w[..., L:].any()
+
+
+@pytest.mark.gpu
+def test_the_smallest_row_weights_are_kept():
+    """Rows that gain nothing (scores far below the largest) keep subnormal weights: eviction tells them apart."""
+    import flash_tree_attn_b200 as fta
+
+    k = torch.full((1, 1, 200, 64), -100.0, device="cuda").half()
+    k[0, 0, 150] = 100.0
+    q = torch.full((1, 1, 1, 64), 10.0, device="cuda").half()
+    bits = torch.arange(1, 201, dtype=torch.int32, device="cuda")
+    w = bits.view(torch.float32).clone().view(1, 1, 200)
+    n = torch.tensor([200], device="cuda")
+    fta.decode_attention(q, k, k, n, row_weights=w)
+    got = w.view(torch.int32)[0, 0]
+    assert w[0, 0, 150] == 1.0 and torch.equal(torch.cat([got[:150], got[151:]]), torch.cat([bits[:150], bits[151:]]))
+    kept = fta.evict_rows(k, k.clone(), n, w, 5, 0)
+    assert kept[0, 0].tolist() == [150, 196, 197, 198, 199]
