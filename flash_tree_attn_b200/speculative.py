@@ -130,7 +130,8 @@ class TreeVerifyAttention(torch.nn.Module):
     sequence, the layout the reference's operator reads (flash_tree_attn.py:238-239).  With
     `page_size` (a multiple of 64) the cache is a pool of pages and a block table, the layout the
     reference's docstring announces (:233); sequence b owns the pages block_table[b], handed out in a
-    shuffled order at construction.
+    shuffled order at construction; a sequence then holds max_seq_len rows rounded up to whole pages, for
+    every method alike.
 
     forward() is the verify step and leaves the cache untouched; commit() appends the accepted
     nodes' keys and values (as given to the last forward) and grows kv_seq_len in place.  decode() is
@@ -172,8 +173,9 @@ class TreeVerifyAttention(torch.nn.Module):
         self.register_buffer("next_position", torch.zeros(max_batch, dtype=torch.int64, device=dev), persistent=False)
         self.register_buffer("inv_freq", None if rotary is None else rotary[0].to(dev), persistent=False)
         self.layout, self.amplitude = ("half", 1.0) if rotary is None else (rotary[1], float(rotary[2]))
-        rows = max_seq_len if table is None else table.size(1) * page_size
-        weights = torch.zeros((max_batch, num_kv_heads, rows), dtype=torch.float32, device=dev) if track_weights else None
+        # what a sequence's cache holds: whole pages, where there are pages
+        self.rows = self.max_seq_len if table is None else table.size(1) * page_size
+        weights = torch.zeros((max_batch, num_kv_heads, self.rows), dtype=torch.float32, device=dev) if track_weights else None
         self.register_buffer("row_weights", weights, persistent=False)
         self._last_kv = None
 
@@ -213,9 +215,9 @@ class TreeVerifyAttention(torch.nn.Module):
         self._last_kv = (k_new, v_new)
         if self.block_table is None:
             return flash_decoding_attention(q, self.k_cache[:B], self.v_cache[:B], k_new, v_new, mask, lens, 64,
-                                            self.max_seq_len, sm_scale=self.sm_scale, kv_group_num=self.G)
+                                            self.rows, sm_scale=self.sm_scale, kv_group_num=self.G)
         return flash_decoding_attention_paged(q, self.k_cache, self.v_cache, self.block_table[:B], k_new, v_new, mask, lens,
-                                              self.max_seq_len, sm_scale=self.sm_scale, kv_group_num=self.G)
+                                              self.rows, sm_scale=self.sm_scale, kv_group_num=self.G)
 
     @torch.no_grad()
     def commit(self, accept_idx: torch.Tensor, accept_len: torch.Tensor) -> None:
@@ -244,7 +246,7 @@ class TreeVerifyAttention(torch.nn.Module):
         q = append_tokens(k, v, q, k_new, v_new, lens, inv_freq=self.inv_freq, layout=self.layout, amplitude=self.amplitude,
                           positions=None if self.inv_freq is None else self.next_position[:B], block_table=table)
         self.next_position[:B] += 1
-        opts = dict(max_seq_len_in_batch=self.max_seq_len, sm_scale=self.sm_scale, kv_group_num=self.G,
+        opts = dict(max_seq_len_in_batch=self.rows, sm_scale=self.sm_scale, kv_group_num=self.G,
                     row_weights=None if self.row_weights is None else self.row_weights[:B])
         if table is None:
             return decode_attention(q, k, v, lens, **opts)

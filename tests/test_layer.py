@@ -1,0 +1,55 @@
+"""TreeVerifyAttention as a decoder's layer uses it: its cache's capacity, commits, casts of the module."""
+import pytest
+import torch
+
+PARENTS = [-1, 0, 0, 1]
+
+
+def _layer(page, max_seq_len, **kw):
+    import flash_tree_attn_b200 as fta
+
+    return fta.TreeVerifyAttention(4, 2, 64, 2, max_seq_len, torch.float16, page_size=page, **kw)
+
+
+def _new(heads, count, g):
+    return torch.randn(2, heads, count, 64, device="cuda", generator=g).half()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,max_seq_len,room", [(64, 100, 128), (128, 130, 256), (None, 100, 100), (64, 128, 128)])
+def test_every_method_has_the_same_capacity(page, max_seq_len, room):
+    """Steps over max_seq_len and over the cache's end: what is stored is attended to, the rest is dropped."""
+    import flash_tree_attn_b200 as fta
+    from oracle.decode_oracle import decode_attention_oracle, sequence_rows
+    from oracle.tree_attention_oracle import tree_attention_oracle
+    from test_decode_attention import _check
+
+    g = torch.Generator(device="cuda").manual_seed(max_seq_len)
+    layer = _layer(page, max_seq_len, track_weights=True)
+    tree = fta.DraftTree(PARENTS)
+    lens = [max_seq_len - 1, 50]
+    layer.load_prefix(*(torch.randn(2, 2, max_seq_len, 64, device="cuda", generator=g).half() for _ in "kv"), lens)
+    table = None if page is None else layer.block_table.cpu()
+    for step in range(room - max_seq_len + 4):
+        q, k, v = _new(4, 1, g), _new(2, 1, g), _new(2, 1, g)
+        before = layer.row_weights.clone()
+        out = layer.decode(q, k, v)
+        stored = lens[0] < room
+        lens = [min(L + 1, room) for L in lens]
+        assert layer.kv_seq_len.tolist() == lens
+        ora = decode_attention_oracle(q, layer.k_cache, layer.v_cache, lens, layer.block_table, 2)
+        _check(out, ora["lse"], None, ora, torch.float16, 64, None, None, room)
+        gained = (layer.row_weights - before)[0, :, lens[0] - 1]
+        assert (gained > 0).all()
+        if stored:
+            kb = sequence_rows(layer.k_cache.cpu(), table, 0, lens[0])
+            assert torch.equal(kb[:, -1], k[0, :, 0].cpu())
+    # the verification of a draft on the full cache sees all of it too
+    q, k, v = _new(4, tree.Q, g), _new(2, tree.Q, g), _new(2, tree.Q, g)
+    out = layer(q, k, v, tree.mask)
+    kc, vc = (torch.zeros(2, 2, room, 64, device="cuda", dtype=torch.float16) for _ in "kv")
+    for b, L in enumerate(lens):
+        for full, t in ((kc, layer.k_cache), (vc, layer.v_cache)):
+            full[b, :, :L] = sequence_rows(t.cpu(), table, b, L).cuda()
+    ora = tree_attention_oracle(q, kc, vc, k, v, tree.mask, torch.tensor(lens, device="cuda"), None, 2)["out"]
+    assert ((out.float() - ora).abs() <= 2e-3 + 2.0 ** -11 * ora.abs()).all()  # the tree operator's own tolerance
