@@ -138,8 +138,9 @@ class TreeVerifyAttention(torch.nn.Module):
     the step of one token without a draft.  The row of a token that finds the cache full is dropped.
 
     rotary: (inv_freq, layout, amplitude) as apply_rotary takes them (`rotary_frequencies` makes the
-    first and the last); queries and new keys are then turned to next_position and on, which counts
-    every token of a sequence, evicted ones too.  Keys given to load_prefix are turned already.
+    first and the last); queries and new keys are then turned to next_position and on.  Keys given to
+    load_prefix are turned already.  next_position [max_batch] int64 counts every token of a sequence,
+    evicted ones too; a layer with neither rotary nor track_weights has none (its rows are its positions).
     track_weights: keep row_weights [max_batch, num_kv_heads, rows] of decode(), which evict() goes by.
     Rows that verification looked at gain nothing; `recent` is there to keep new rows until decode()
     has looked at them."""
@@ -170,7 +171,9 @@ class TreeVerifyAttention(torch.nn.Module):
         self.register_buffer("v_cache", torch.zeros_like(k), persistent=False)
         self.register_buffer("kv_seq_len", torch.zeros(max_batch, dtype=torch.int32, device=dev), persistent=False)
         self.register_buffer("block_table", table, persistent=False)
-        self.register_buffer("next_position", torch.zeros(max_batch, dtype=torch.int64, device=dev), persistent=False)
+        # the next token's position, where it can differ from kv_seq_len or is asked for; else None
+        counted = rotary is not None or track_weights
+        self.register_buffer("next_position", torch.zeros(max_batch, dtype=torch.int64, device=dev) if counted else None, persistent=False)
         self.register_buffer("inv_freq", None if rotary is None else rotary[0].to(dev), persistent=False)
         self.layout, self.amplitude = ("half", 1.0) if rotary is None else (rotary[1], float(rotary[2]))
         # what a sequence's cache holds: whole pages, where there are pages
@@ -196,7 +199,8 @@ class TreeVerifyAttention(torch.nn.Module):
                     self.k_cache[pg, :, : r1 - r0] = k[b, :, r0:r1]
                     self.v_cache[pg, :, : r1 - r0] = v[b, :, r0:r1]
         self.kv_seq_len[:B] = torch.as_tensor(list(lens), dtype=torch.int32)
-        self.next_position[:B] = torch.as_tensor(list(lens), dtype=torch.int64)
+        if self.next_position is not None:
+            self.next_position[:B] = torch.as_tensor(list(lens), dtype=torch.int64)
         if self.row_weights is not None:
             self.row_weights[:B] = 0.0
 
@@ -232,7 +236,8 @@ class TreeVerifyAttention(torch.nn.Module):
         else:
             commit_accepted(self.k_cache, self.v_cache, k_new, v_new, self.kv_seq_len[:B], accept_idx, accept_len,
                             kv_group_num=self.G, block_table=self.block_table[:B])
-        self.next_position[:B] += accept_len.to(self.next_position.device).clamp(0, accept_idx.size(1))
+        if self.next_position is not None:
+            self.next_position[:B] += accept_len.to(self.next_position.device).reshape(-1).clamp(0, accept_idx.size(1))
 
     @torch.no_grad()
     def decode(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
@@ -245,7 +250,8 @@ class TreeVerifyAttention(torch.nn.Module):
         k, v = (self.k_cache[:B], self.v_cache[:B]) if table is None else (self.k_cache, self.v_cache)
         q = append_tokens(k, v, q, k_new, v_new, lens, inv_freq=self.inv_freq, layout=self.layout, amplitude=self.amplitude,
                           positions=None if self.inv_freq is None else self.next_position[:B], block_table=table)
-        self.next_position[:B] += 1
+        if self.next_position is not None:
+            self.next_position[:B] += 1
         opts = dict(max_seq_len_in_batch=self.rows, sm_scale=self.sm_scale, kv_group_num=self.G,
                     row_weights=None if self.row_weights is None else self.row_weights[:B])
         if table is None:

@@ -53,3 +53,34 @@ def test_every_method_has_the_same_capacity(page, max_seq_len, room):
             full[b, :, :L] = sequence_rows(t.cpu(), table, b, L).cuda()
     ora = tree_attention_oracle(q, kc, vc, k, v, tree.mask, torch.tensor(lens, device="cuda"), None, 2)["out"]
     assert ((out.float() - ora).abs() <= 2e-3 + 2.0 ** -11 * ora.abs()).all()  # the tree operator's own tolerance
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [None, 64])
+@pytest.mark.parametrize("kind", ["plain", "rotary", "weights"])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_accepted_lengths_of_any_shape(page, kind, dtype):
+    """commit takes accept_len as commit_accepted does: as many elements as sequences.  Lengths past the path count
+    as the path's, negative ones as none."""
+    import flash_tree_attn_b200 as fta
+    from oracle.decode_oracle import sequence_rows
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    kw = {"rotary": dict(rotary=(fta.rotary_frequencies(64)[0], "half", 1.0)), "weights": dict(track_weights=True)}.get(kind, {})
+    tree = fta.DraftTree(PARENTS)
+    idx = torch.tensor([[0, 1, 3], [0, 2, 0]], dtype=torch.int32, device="cuda")
+    for n, counts in (([[2], [1]], (2, 1)), ([[9], [-4]], (3, 0)), ([3, 2], (3, 2))):
+        layer = _layer(page, 128, **kw)
+        layer.load_prefix(*(torch.randn(2, 2, 50, 64, device="cuda", generator=g).half() for _ in "kv"), [50, 7])
+        q, k, v = _new(4, tree.Q, g), _new(2, tree.Q, g), _new(2, tree.Q, g)
+        layer(q, k, v, tree.mask, depth=tree.depth)
+        layer.commit(idx, torch.tensor(n, dtype=dtype, device="cuda"))
+        want = [50 + counts[0], 7 + counts[1]]
+        assert layer.kv_seq_len.tolist() == want
+        assert (layer.next_position is None) if kind == "plain" else (layer.next_position.tolist() == want)
+        table = None if page is None else layer.block_table.cpu()
+        for b, c in enumerate(counts):
+            rows = sequence_rows(layer.v_cache.cpu(), table, b, want[b])
+            assert torch.equal(rows[:, want[b] - c:], v[b][:, idx[b, :c].long()].cpu())
+    out = layer.decode(_new(4, 1, g), _new(2, 1, g), _new(2, 1, g))
+    assert out.shape == (2, 4, 1, 64) and layer.kv_seq_len.tolist() == [want[0] + 1, want[1] + 1]
