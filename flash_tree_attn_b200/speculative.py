@@ -182,6 +182,17 @@ class TreeVerifyAttention(torch.nn.Module):
         self.register_buffer("row_weights", weights, persistent=False)
         self._last_kv = None
 
+    def _apply(self, fn, *args, **kwargs):
+        """A cast of the module (`.half()`, `.to(dtype)`) is for the caches: frequencies stay in 64 bits and row
+        weights in 32, as the operators take them.  As integers they only move."""
+        kept = {name: self._buffers[name] for name in ("inv_freq", "row_weights") if self._buffers[name] is not None}
+        super()._apply(fn, *args, **kwargs)
+        for name, t in kept.items():
+            if self._buffers[name].dtype is not t.dtype:
+                as_int = torch.int64 if t.dtype is torch.float64 else torch.int32
+                self._buffers[name] = fn(t.view(as_int)).view(t.dtype)
+        return self
+
     @torch.no_grad()
     def load_prefix(self, k: torch.Tensor, v: torch.Tensor, lens: Sequence[int]) -> None:
         """Fill the cache after prefill: k, v [bsz, num_kv_heads, L, head_dim], lens[b] <= L rows count."""

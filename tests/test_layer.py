@@ -84,3 +84,42 @@ def test_accepted_lengths_of_any_shape(page, kind, dtype):
             assert torch.equal(rows[:, want[b] - c:], v[b][:, idx[b, :c].long()].cpu())
     out = layer.decode(_new(4, 1, g), _new(2, 1, g), _new(2, 1, g))
     assert out.shape == (2, 4, 1, 64) and layer.kv_seq_len.tolist() == [want[0] + 1, want[1] + 1]
+
+
+def test_casts_leave_frequencies_and_weights_as_they_are():
+    import flash_tree_attn_b200 as fta
+
+    f, _ = fta.rotary_frequencies(64, device="cpu")
+    for cast, dtype in ((lambda m: m.half(), torch.float16), (lambda m: m.to(torch.bfloat16), torch.bfloat16),
+                        (lambda m: torch.nn.Sequential(m).to("cpu", torch.bfloat16)[0], torch.bfloat16), (lambda m: m.double().half(), torch.float16)):
+        layer = fta.TreeVerifyAttention(4, 2, 64, 2, 100, torch.float16, device="cpu", rotary=(f, "half", 1.0), track_weights=True)
+        layer.row_weights.normal_()
+        weights = layer.row_weights.clone()
+        got = cast(layer)
+        assert got is layer and layer.k_cache.dtype is dtype and layer.v_cache.dtype is dtype
+        assert layer.inv_freq.dtype is torch.float64 and torch.equal(layer.inv_freq, f)
+        assert layer.row_weights.dtype is torch.float32 and torch.equal(layer.row_weights, weights)
+        assert layer.kv_seq_len.dtype is torch.int32 and layer.next_position.dtype is torch.int64
+    layer.to("meta")
+    assert layer.inv_freq.is_meta and layer.row_weights.is_meta and layer.inv_freq.dtype is torch.float64
+    layer.to_empty(device="cpu").half()
+    assert layer.inv_freq.dtype is torch.float64 and layer.row_weights.shape == (2, 2, 100)
+    plain = fta.TreeVerifyAttention(4, 2, 64, 2, 100, torch.float16, device="cpu").to(torch.bfloat16)
+    assert plain.inv_freq is None and plain.row_weights is None and plain.k_cache.dtype is torch.bfloat16
+
+
+@pytest.mark.gpu
+def test_a_cast_layer_steps_on():
+    import flash_tree_attn_b200 as fta
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+    f, amplitude = fta.rotary_frequencies(64, scaling="ramp", factor=4.0)
+    tree = fta.DraftTree(PARENTS)
+    layers = [_layer(64, 128, rotary=(f, "half", amplitude), track_weights=True) for _ in range(2)]
+    torch.nn.ModuleList(layers[1:]).half().cuda()
+    prefix = [torch.randn(2, 2, 50, 64, device="cuda", generator=g).half() for _ in "kv"]
+    for layer in layers:
+        layer.load_prefix(*prefix, [50, 7])
+    one, draft = [_new(h, 1, g) for h in (4, 2, 2)], [_new(h, tree.Q, g) for h in (4, 2, 2)]
+    got = [(layer.decode(*one), layer(*draft, tree.mask, depth=tree.depth), layer.evict(20, 3), layer.row_weights) for layer in layers]
+    assert all(torch.equal(a, b) for a, b in zip(*got))
