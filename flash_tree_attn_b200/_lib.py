@@ -217,13 +217,16 @@ def load():
             "(there is no non-CUDA fallback for this operator)"
         )
     lib = C.CDLL(LIB_PATH)
+    rebuild = "rebuild it with `python -m flash_tree_attn_b200.build`"
+    missing = [name for name in SYMBOLS if not hasattr(lib, name)]
+    if missing:  # an older library of the same ABI version: entries are added without a new one
+        raise FtaLibraryMissing(f"{LIB_PATH} lacks {', '.join(missing)}: {rebuild}")
     for name, (res, args) in SYMBOLS.items():
-        fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
+        fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
     if lib.fta_version() != ABI_VERSION:
-        raise FtaLibraryMissing(f"{LIB_PATH} has ABI version {lib.fta_version()}, this package binds version {ABI_VERSION}: "
-                                "rebuild it with `python -m flash_tree_attn_b200.build`")
+        raise FtaLibraryMissing(f"{LIB_PATH} has ABI version {lib.fta_version()}, this package binds version {ABI_VERSION}: {rebuild}")
     _lib = lib
     return lib
 

@@ -32,7 +32,8 @@ extern "C" {
 #endif
 
 /* 101: FtaExchangeParams.done points at two int32s (scatter form); stage 2 is a programmatic
-   dependent launch.  100: first version. */
+   dependent launch.  100: first version.  A new version is a change that breaks a caller; entries are
+   added without one, so a caller asks the loaded library for those it needs. */
 #define FTA_VERSION 101
 
 /* ---- error codes ------------------------------------------------------------------- */
