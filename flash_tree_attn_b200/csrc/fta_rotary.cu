@@ -2,9 +2,10 @@
 //
 // Angles.  A cosine needs its angle modulo one turn, and position * frequency in 32 bits has lost that
 // after some 10^5 positions.  So a pair's frequency is kept as a 64-bit fraction of a turn, and
-// position * fraction, modulo 2^64, IS the angle modulo one turn: an integer product, exact but for
-// the fraction's own rounding (2^-64 turns a position).  Its top 32 bits, as a signed number of
-// half-turns, go to sincospi.
+// position * fraction, modulo 2^64, IS the angle modulo one turn: an integer product, exact but for what the
+// fraction is off by: 2^-52 of inv_freq / 2 pi (1 / 2 pi and the product with it are rounded in 64 bits) and
+// 2^-65 of a turn.  At frequency 1 that is below 2^-23 of a turn at position 2^31, 2^-14 at 2^40.  The product's top 32
+// bits, as a signed number of half-turns, go to sincospi in 24 bits: 2^-26 of a turn.
 //
 // What bounds it: each element is read once and written once; nothing else moves but 8 bytes per
 // pair.  A block works out the cosines and sines of its tokens once, in shared memory, for all heads, while

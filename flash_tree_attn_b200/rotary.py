@@ -1,9 +1,10 @@
 """Rotary positions of queries and keys, and the append of new tokens to the cache.
 
 Frequencies are data: any scheme for long contexts is a list of radians per position, one for each
-pair, in 64 bits (`rotary_frequencies` makes the usual ones).  A position is an integer of any size;
-angles are taken modulo one turn in whole numbers, so far positions lose nothing.  All arithmetic
-happens in libfta.so.
+pair, in 64 bits (`rotary_frequencies` makes the usual ones).  Positions are integers, and angles are
+taken modulo one turn in whole numbers: an angle is off by |position| * (inv_freq / 2 pi * 2^-52 + 2^-65)
+of a turn and 2^-26 of a turn for 32-bit cosines, so that positions up to 2^28 lose less than 32 bits
+hold.  All arithmetic happens in libfta.so.
 """
 from __future__ import annotations
 

@@ -311,8 +311,9 @@ int fta_decode_token(const FtaTokenParams* p, void* stream);
  *   rows at or past ctx and rows of pages outside [0, n_pages) are dropped; kv_seq_len[b] grows by Q
  *   in place, at most to ctx.  positions NULL: kv_seq_len[b] before the call.  n_freq 0 turns nothing;
  *   q may then be NULL with H = 0.
- * inv_freq is [n_freq] float64, finite.  An angle is position * (inv_freq / 2 pi) modulo one turn, exact
- * but for the quotient's rounding in 64 bits, then rounded to 2^-32 of a turn.
+ * inv_freq is [n_freq] float64, finite.  An angle is position * (inv_freq / 2 pi) modulo one turn.  The quotient is
+ * off by 2^-52 of itself and 2^-65 of a turn at most, and so the angle by |position| times that; the
+ * product is exact, and its result rounded to 2^-26 of a turn.
  */
 #define FTA_ROTARY_HALF 0
 #define FTA_ROTARY_INTERLEAVED 1
