@@ -211,6 +211,10 @@ __host__ __device__ __forceinline__ bool fta_row(const FtaParams& p, const FtaGe
   return hh < g.hpt && gi < (p.H / p.Hkv) && qi < p.Q;
 }
 
+// SMs of a B200.  Rules that choose between forms of a kernel by how many blocks they make go by it, as they were
+// measured there; plans that deal work out to resident blocks ask the device.
+constexpr int kFtaSms = 148;
+
 // Keeps the text of a CUDA error for fta_last_cuda_error and returns FTA_E_CUDA (fta_api.cu).
 int fta_cuda_fail(cudaError_t e);
 

@@ -299,9 +299,9 @@ extern "C" int fta_evict_rows(const FtaEvictParams* p, void* stream) {
   const long long units = (long long)p->B * p->Hkv * 2;
   const int width = p->D / 8;
   int blocks = 1, slices = 1;
-  while (units * blocks < 3 * 148 && blocks < 8) blocks *= 2;
-  while (units * blocks * slices < 4 * 148 && blocks == 8 && width / slices > 4) slices *= 2;
-  while (units * blocks * slices < 2 * 148 && width / slices > 2) slices *= 2;
+  while (units * blocks < 3 * kFtaSms && blocks < 8) blocks *= 2;
+  while (units * blocks * slices < 4 * kFtaSms && blocks == 8 && width / slices > 4) slices *= 2;
+  while (units * blocks * slices < 2 * kFtaSms && width / slices > 2) slices *= 2;
   e = fta_launch_after(evict_move_kernel, dim3(p->B * p->Hkv * blocks, 2, slices), kMove, 0, st, blocks, *p, width / slices, blocks);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
 }

@@ -513,7 +513,7 @@ int run_with(const FtaLogprobParams& p, cudaStream_t st) {
   const int chunks = p.vocab / Vec<T>::n, pieces = chunks > 0 ? fta_cdiv(chunks, THREADS * kChunks) : 1;
   // Blocks per row: enough to fill the machine, and no more.  A wave of blocks lasts as long as its
   // rounds, and about one round more for the start and the end of a block, another one for a cluster's join.
-  const int slots = 148 * Cfg<THREADS>::kBlocks;
+  const int slots = kFtaSms * Cfg<THREADS>::kBlocks;
   int blocks = 1, rounds = pieces;
   long long least = 0x7fffffffffffffffLL;
   for (int n = 1; n <= kMostBlocks && n <= pieces; ++n) {
@@ -532,8 +532,8 @@ int run(const FtaLogprobParams& p, cudaStream_t st) {
   // maximum at best): a warp's 64 chunks then hold twice or three times k for k up to 16, two warps' 128 for k
   // up to 40; beyond, the lists would overflow, unless they hold all of a row, and the exact bound be searched.
   const int chunks = p.vocab / Vec<T>::n;
-  if (p.rows > 148 * 4 && chunks <= 32 * kChunks && p.top_k <= 16) return run_with<T, 32>(p, st);
-  if (p.rows > 148 * 4 && chunks <= (p.top_k <= 40 ? 64 * kChunks : Cfg<64>::kListedChunks)) return run_with<T, 64>(p, st);
+  if (p.rows > kFtaSms * 4 && chunks <= 32 * kChunks && p.top_k <= 16) return run_with<T, 32>(p, st);
+  if (p.rows > kFtaSms * 4 && chunks <= (p.top_k <= 40 ? 64 * kChunks : Cfg<64>::kListedChunks)) return run_with<T, 64>(p, st);
   return run_with<T, 256>(p, st);
 }
 

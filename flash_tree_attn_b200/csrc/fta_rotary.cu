@@ -202,7 +202,7 @@ int launch(const FtaRotaryParams* p, cudaStream_t st) {
   if (int rc = check(p, APPEND)) return rc;
   // Four tokens a block once that still leaves every SM several blocks: they share the start of a block
   // (length, page, a barrier) and a head's rows of four tokens are one piece of memory.
-  const bool four = p->Q >= 4 && (long long)p->B * p->Q >= 148 * 16;
+  const bool four = p->Q >= 4 && (long long)p->B * p->Q >= kFtaSms * 16;
   const dim3 grid(four ? (p->Q + 3) / 4 : p->Q, p->B);
   const int bits = p->D == 32 ? 1 : p->D == 64 ? 2 : p->D == 128 ? 3 : 4;
   const bool f16 = p->dtype == FTA_DTYPE_F16;

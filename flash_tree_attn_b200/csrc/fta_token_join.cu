@@ -257,9 +257,11 @@ int geometry(const FtaTokenParams& p, FtaGeom& g) {
   g.lanes = g.mtiles > 1 && g.grid >= g.mtiles ? g.mtiles : 1;
   // Short caches: one launch, a cluster of blocks per unit that joins without a second kernel.  It shares
   // out each unit's tiles evenly but not those of different lengths, so no block may get more than 8 tiles
-  // (16 of a single sequence), and all clusters are resident at once.  On the GPU, clusters against the
-  // BALANCED plan, 32/8 heads of 128: one sequence of 1000 rows 4.7 and 8.3 us, of 4000 8.1 and 11.5, of 16000
-  // 22.1 and 22.9; 8 sequences of 2000 rows 14.5 and 18.7.
+  // (16 of a single sequence, 8192 rows in clusters of 8), and all clusters are resident at once.  The rule goes
+  // by the cache's capacity or the window: lengths are on the device, so a short sequence in a large cache takes
+  // the BALANCED plan.  On the GPU, clusters against the BALANCED plan, 32/8 heads of 128: one sequence of 1000
+  // rows 4.7 and 8.3 us, of 4000 8.1 and 11.5; 8 sequences of 2000 rows 14.5 and 18.7.  Without the limit one
+  // sequence of 16000 rows took 22.1 and 22.9: little was left of the gain.
   if (p.grid_override == 0 && !p.row_weights && p.B <= 4096) {
     const int rows = p.window > 0 && p.window < p.ctx ? p.window + FTA_TILE - 1 : p.ctx;
     const int tiles = rows > 0 ? fta_cdiv(rows, FTA_TILE) : 1;
@@ -303,7 +305,7 @@ extern "C" int fta_decode_token(const FtaTokenParams* p, void* stream) {
   while (weights && fta_cdiv(p->ctx, chunk) > 65535) chunk *= 2;  // a grid's second dimension ends there
   const int chunks = weights ? fta_cdiv(p->ctx, chunk) : 0;
   // a block per head where there are few KV heads: then a unit has many pieces
-  const int shares = p->B * p->Hkv < 148 ? p->H / p->Hkv : 1;
+  const int shares = p->B * p->Hkv < kFtaSms ? p->H / p->Hkv : 1;
   const dim3 grid(p->B * p->Hkv, shares > chunks ? shares : chunks);
   e = fta_launch_after(token_join_kernel, grid, kThreads, 0, st, 1, *p, g, shares, chunk);
   return e == cudaSuccess ? FTA_OK : fta_cuda_fail(e);
