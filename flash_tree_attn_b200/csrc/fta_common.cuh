@@ -296,6 +296,12 @@ template <> struct FtaType<__half> {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  // towards zero; a NaN stays one
+  static __device__ __forceinline__ uint32_t pack_down(float a, float b) {
+    uint32_t y;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(b), "f"(a));
+    return y;
+  }
   static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
   static __device__ __forceinline__ __half from_float(float a) { return __float2half_rn(a); }
 };
@@ -305,7 +311,9 @@ template <> struct FtaType<__nv_bfloat16> {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
-  static __device__ __forceinline__ float2 unpack(uint32_t x) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x)); }
+  // towards zero; a NaN as the exponential makes it (all ones) stays one
+  static __device__ __forceinline__ uint32_t pack_down(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+  static __device__ __forceinline__ float2 unpack(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float a) { return __float2bfloat16_rn(a); }
 };
 
