@@ -199,6 +199,9 @@ int check_sizes(const FtaTokenParams* p) {
   if (p->dtype != FTA_DTYPE_F16 && p->dtype != FTA_DTYPE_BF16) return FTA_E_BADARG;
   if (p->grid_override < 0) return FTA_E_BADARG;
   if (p->B > FTA_MAX_BATCH || p->H / p->Hkv > FTA_MAX_GROUP || p->ctx > FTA_MAX_ROWS) return FTA_E_UNSUPPORTED;
+  // the plan counts all sequences' 64-row tiles, and a few more each, in 32 bits
+  const int rows = p->window > 0 && p->window < p->ctx ? p->window + FTA_TILE : p->ctx;
+  if ((long long)p->B * (fta_cdiv(rows, FTA_TILE) + 8) > 0x7fffffffLL) return FTA_E_UNSUPPORTED;
   return FTA_OK;
 }
 

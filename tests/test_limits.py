@@ -20,6 +20,12 @@ def test_attention_refuses_longer_caches(fta_lib):
     from test_decode_attention import _fake
 
     assert fta_lib.fta_decode_token(C.byref(_fake(ctx=MOST + 1)), None) == _lib.FTA_E_UNSUPPORTED
+    # and batches whose 64-row tiles a 32-bit number does not count; a window keeps them few
+    many = dict(B=8192, ctx=2 ** 24, bt_sb=2 ** 18)
+    assert fta_lib.fta_decode_token(C.byref(_fake(**many)), None) == _lib.FTA_E_UNSUPPORTED
+    assert fta_lib.fta_decode_token_workspace_bytes(C.byref(_fake(**many))) == -_lib.FTA_E_UNSUPPORTED
+    assert fta_lib.fta_decode_token_workspace_bytes(C.byref(_fake(**many, window=4096))) > 0
+    assert fta_lib.fta_decode_token_workspace_bytes(C.byref(_fake(B=8192, ctx=2 ** 23))) > 0
 
 
 @pytest.mark.gpu
