@@ -173,7 +173,10 @@ def decode_attention(q, k_cache, v_cache, kv_seq_len, *, max_seq_len_in_batch: O
             Distances count cache rows, so this does not go with evict_rows, which closes up gaps.
         window: only the last `window` rows of a sequence are seen.
         row_weights: [bsz, num_kv_heads, ctx] fp32, updated in place: row r of a KV head gains the
-            softmax weights that the group's query heads gave it (what evict_rows goes by).
+            softmax weights that the group's query heads gave it (what evict_rows goes by).  The call then
+            keeps every score until it ends, 4 bytes x bsz x num_heads x ctx of scratch by the cache's
+            capacity, not the lengths: 2 GB for 64 sequences of 131072 rows and 64 heads.
+            max_seq_len_in_batch bounds that too.
         return_lse: also return the fp32 natural-log LSE [bsz, num_heads, 1].
 
     An empty sequence gives zeros and an LSE of -inf.  Asynchronous on the current stream of q's

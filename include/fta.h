@@ -258,7 +258,9 @@ int fta_commit_accepted(const FtaCommitParams* p, void* stream);
  * The reference has no such entry; shapes, strides and the page table are FtaParams' with Q = 1.
  *   row_weights  optional fp32 [B, Hkv, ctx], unit stride along ctx: row r of KV head kvh gains the
  *                softmax weights that the group's G query heads gave it (updated in place, by one
- *                thread per row in a fixed order: equal inputs give equal bits)
+ *                thread per row in a fixed order: equal inputs give equal bits).  The workspace then has
+ *                room for every score, 4 * B * H * ctx bytes, whatever the lengths are; ctx may be less than
+ *                the cache holds where no sequence is longer
  * ctx is at most FTA_MAX_ROWS.  An empty sequence gives out = 0, lse = -inf.  A page index outside [0, n_pages) takes the rows
  * of that page out of the attention; nothing outside the pool is read.
  */
